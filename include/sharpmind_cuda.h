@@ -364,6 +364,50 @@ SMC_API int smc_kv_restore(smc_ctx *ctx, smc_kv *kv, const void *host_k, const v
 SMC_API int smc_sdpa_kv_dev(smc_ctx *ctx, const smc_kv *kv, const float *d_q, float *d_out, int batch, int heads, int seqLen,
                             float scale, void *stream);
 
+/* ---- paged KV cache in 8 bits ------------------------------------------------------------------
+ * Keys and values of one attention layer for sequences of their own lengths.  No counterpart in the reference, whose caches
+ * (IKVCache.cs) are contiguous and hold lock-step sequences; beside smc_kv_* above.
+ * The memory is the caller's: `pages` pages of `page` tokens (16, 32 or 64); of page i and head h, keys [page, head_dim] and values
+ * [head_dim, page] as e4m3 codes, and two scales.  head_dim 64 or 128.  A block is a page's tokens of one head, keys and values apart:
+ *   scale = 2^k, the smallest (k >= -40) under which every magnitude that entered the block since its first token fits 448 2^k
+ *   code  = e4m3(x / scale) to nearest even;  a code stands for code * scale
+ * The first token of a page starts its blocks over; where a later one makes a scale grow, the codes that are there are rounded to it.  A block
+ * that an infinite or undefined value entered has the scale NaN: rows that see one of its tokens come out as NaN, other rows do not.
+ * Position p of sequence s is token p % page of page table[s * width + p / page].  `lengths` counts the tokens of a sequence, new ones included;
+ * rows row_start[s] .. row_start[s + 1] - 1 of a call are its last ones (row_start null: one row each).  Rows from row_start[batch] on are
+ * neither read nor written.  These arrays are on the device, so a captured CUDA graph serves what they hold when it is replayed.
+ * A page that a call writes belongs to one sequence; pages that are only read may be shared.  The calls queue on `stream` and keep nothing
+ * in the context.  A page number outside of [0, pages), a length outside of the table or of the rotation's tables, or rows outside of the
+ * call's raise smc_device_status (value 6): nothing is read or written outside of the arrays, the results of that sequence are not defined. */
+typedef struct smc_paged_kv {
+    void *k, *v;   /* [pages, kv_heads, page, head_dim], [pages, kv_heads, head_dim, page], 16-byte aligned */
+    float *scales; /* [pages, kv_heads, 2]: keys, values */
+    int pages, kv_heads, page, head_dim;
+} smc_paged_kv;
+typedef struct smc_paged_seqs {
+    const int *table;     /* [batch, width] */
+    const int *lengths;   /* [batch] */
+    const int *row_start; /* [batch + 1], or null */
+    int batch, width, rows;
+} smc_paged_seqs;
+/* KVCache.Update (KVCache.cs:84-150) for new rows d_k, d_v [rows, kv_heads, head_dim] (dtype SMC_F32 or SMC_BF16; strides in elements between rows,
+ * so that they may be parts of a joined product; 16-byte aligned), with RoPE.Apply (RoPE.cs:168-259) on the way where d_cos / d_sin
+ * [table_rows, rope_dim / 2] are given: keys are rotated to their positions, and queries d_q [rows, heads, head_dim] (may be null) to d_q_out
+ * (contiguous; may be d_q itself if that is).  neox as for smc_rope_dev.  rope_dim % 8 == 0. */
+SMC_API int smc_paged_update_dev(smc_ctx *ctx, const smc_paged_kv *kv, const smc_paged_seqs *seqs, int dtype, const void *d_k, long long k_stride,
+                                 const void *d_v, long long v_stride, const void *d_q, long long q_stride, void *d_q_out, int heads, const float *d_cos,
+                                 const float *d_sin, int rope_dim, int table_rows, int neox, void *stream);
+/* Values of n listed pages, d_k and d_v [n, page, kv_heads, head_dim] fp32 or bfloat16 (where a code times its scale is exact). */
+SMC_API int smc_paged_read_dev(smc_ctx *ctx, const smc_paged_kv *kv, const int *d_pages, int n, int dtype, void *d_k, void *d_v, void *stream);
+/* Causal attention of every sequence's rows over its pages (AttentionLayer.Forward's loop, AttentionLayer.cs:326-413, as smc_sdpa_kv_dev): d_q
+ * [rows, heads, head_dim] with a row stride in elements, d_out contiguous, both of `dtype`.  window > 0: position i sees
+ * i - window + 1 .. i.  A row that sees no key gets zeros.  max_rows bounds the rows of a sequence (one with more raises status 6) and max_len says how
+ * long the sequences may be; both are known to the host and choose and size the launch.  d_work: smc_paged_attention_work bytes (-1 for
+ * bad arguments), 16-byte aligned, used by this call alone until it has completed. */
+SMC_API int64_t smc_paged_attention_work(smc_ctx *ctx, const smc_paged_kv *kv, int batch, int heads, int max_rows, int max_len);
+SMC_API int smc_paged_attention_dev(smc_ctx *ctx, const smc_paged_kv *kv, const smc_paged_seqs *seqs, int dtype, const void *d_q, long long q_stride, void *d_out,
+                                    int heads, float scale, int window, int max_rows, int max_len, void *d_work, long long work_bytes, void *stream);
+
 /* ---- one decode step of a Llama/Qwen-shaped decoder -------------------------------------------
  * What Transformer.ForwardLastLogits computes for [batch, 1] token ids (SharpMind.Model/Transformer.cs:417-463
  * -> DecoderArch.Forward Arch/DecoderArch.cs:115-134 -> UnhookedTransformerBlock.Forward

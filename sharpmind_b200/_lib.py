@@ -79,6 +79,12 @@ SIGNATURES = {
     "smc_kv_snapshot": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, C.POINTER(c_int)]),
     "smc_kv_restore": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int]),
     "smc_sdpa_kv_dev": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_void_p]),
+    "smc_paged_update_dev": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int,
+                                     c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
+    "smc_paged_read_dev": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "smc_paged_attention_work": (c_int64, [c_void_p, c_void_p, c_int, c_int, c_int, c_int]),
+    "smc_paged_attention_dev": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int, c_float, c_int, c_int, c_int,
+                                        c_void_p, c_int64, c_void_p]),
     "smc_model_create": (c_int, [c_void_p, c_void_p, c_int, _pp]),
     "smc_model_destroy": (c_int, [c_void_p, c_void_p]),
     "smc_model_kv": (c_int, [c_void_p, c_void_p, _pp, _pp]),

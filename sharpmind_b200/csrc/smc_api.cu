@@ -262,7 +262,7 @@ int smc_device_status(smc_ctx *ctx, int *status)
     SMC_CUDA(ctx, cudaMemcpy(status, ctx->d_status, sizeof(int), cudaMemcpyDeviceToHost));
     if (*status) {
         SMC_CUDA(ctx, cudaMemset(ctx->d_status, 0, sizeof(int)));
-        return smc_fail(ctx, SMC_E_CUDA, "a kernel gave up a bounded wait, or (status 5) a sequence ran past max_seq (status %d): its outputs are invalid", *status);
+        return smc_fail(ctx, SMC_E_CUDA, "a kernel gave up a bounded wait, or (status 5) a sequence ran past max_seq, or (status 6) a paged cache was given a page, length or row out of range (status %d): its outputs are invalid", *status);
     }
     return SMC_OK;
 }

@@ -1,0 +1,92 @@
+// What the kernels of the paged key/value cache share: the cache and its sequences as kernels see them, rows and positions, and the 8-bit codes.
+#pragma once
+#include <cuda_fp8.h>
+
+#include "smc_mma.cuh"
+
+// status word of smc_device_status: a page number, length or position outside of what the call was given
+constexpr int SMC_STATUS_PAGED = 6;
+
+struct smc_paged_view {
+    uint8_t *k, *v;  // [pages, kvh, page, hd], [pages, kvh, hd, page] e4m3 codes
+    float *scales;   // [pages, kvh, 2]
+    int pages, kvh, shift;  // page = 1 << shift
+    const int *table, *lengths, *row_start;
+    int batch, width, rows;
+};
+
+#ifdef __CUDACC__
+// Rows [r0, r0 + n) of sequence s sit at positions [len - n, len); whatever the device arrays hold, rows stay inside of [0, rows) and
+// positions inside of the table.
+struct smc_paged_seq {
+    int r0, n, len;
+    bool bad;
+};
+__device__ __forceinline__ smc_paged_seq smc_paged_sequence(const smc_paged_view &c, int s)
+{
+    smc_paged_seq q;
+    int a = s, b = s + 1;
+    if (c.row_start) a = c.row_start[s], b = c.row_start[s + 1];
+    q.r0 = min(max(a, 0), c.rows);
+    q.n = min(max(b, q.r0), c.rows) - q.r0;
+    const int len = c.lengths[s];
+    const long long most = (long long)c.width << c.shift;
+    q.len = (int)min((long long)max(len, 0), most);
+    q.bad = a < 0 || b < a || b > c.rows || len < 0 || len > most;
+    return q;
+}
+// page `i` of sequence s, or -1
+__device__ __forceinline__ int smc_paged_page(const smc_paged_view &c, int s, int i)
+{
+    const int id = i < c.width ? c.table[(size_t)s * c.width + i] : -1;
+    return id >= 0 && id < c.pages ? id : -1;
+}
+// the sequence that row r of the call belongs to (-1: a row behind the last one)
+__device__ __forceinline__ int smc_paged_row_sequence(const smc_paged_view &c, int r)
+{
+    if (!c.row_start) return r < c.batch ? r : -1;
+    int lo = 0, hi = c.batch;  // the last s with row_start[s] <= r
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (c.row_start[mid] <= r) lo = mid;
+        else hi = mid;
+    }
+    return c.row_start[lo] <= r && r < c.row_start[lo + 1] ? lo : -1;
+}
+
+// two codes as halves (exact: e4m3 is a subset of fp16)
+__device__ __forceinline__ uint32_t smc_e4m3x2_half2(uint32_t two)
+{
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((unsigned short)two));
+    return h;
+}
+__device__ __forceinline__ void smc_e4m3x4_float(uint32_t w, float (&f)[4])
+{
+    const uint32_t a = smc_e4m3x2_half2(w & 0xFFFFu), b = smc_e4m3x2_half2(w >> 16);
+    const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&a)), y = __half22float2(*reinterpret_cast<const __half2 *>(&b));
+    f[0] = x.x, f[1] = x.y, f[2] = y.x, f[3] = y.y;
+}
+// four values as codes, round to nearest even; the first in the low byte
+__device__ __forceinline__ uint32_t smc_float_e4m3x4(const float (&f)[4])
+{
+    unsigned short a, b;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(a) : "f"(f[1]), "f"(f[0]));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b) : "f"(f[3]), "f"(f[2]));
+    return (uint32_t)a | ((uint32_t)b << 16);
+}
+// Four neighbouring elements of a row as floats, and floats as elements
+template <typename T> __device__ __forceinline__ void smc_paged_load4(const T *p, float (&f)[4]) { load_v<T, 4>(p, f); }
+template <typename T> __device__ __forceinline__ void smc_paged_store4(T *p, const float (&f)[4]) { store_v<T, 4>(p, f); }
+#endif
+
+// Launchers of the attention's forms (smc_paged_attend.cu)
+struct smc_ctx;
+struct smc_paged_query {
+    const void *q;
+    long long q_stride;
+    void *out;
+    int bf16, heads, hd, window, max_rows, max_len;
+    float scale;
+};
+int smc_launch_paged_attend(smc_ctx *, const smc_paged_view &, const smc_paged_query &, cudaStream_t s);

@@ -29,6 +29,23 @@ public unsafe struct SmcModelDesc
     public int KvDtype;                               // 0 = fp32 cache, 8 = Q8_0 rows
 }
 
+/// <summary>Field-for-field mirror of <c>smc_paged_kv</c>: a paged key/value cache in the caller's device memory.</summary>
+[StructLayout(LayoutKind.Sequential)]
+public struct SmcPagedKv
+{
+    public nint K, V;      // e4m3 codes [pages, kvHeads, page, headDim], [pages, kvHeads, headDim, page]
+    public nint Scales;    // device float* [pages, kvHeads, 2]
+    public int Pages, KvHeads, Page, HeadDim;
+}
+
+/// <summary>Field-for-field mirror of <c>smc_paged_seqs</c> (device int arrays).</summary>
+[StructLayout(LayoutKind.Sequential)]
+public struct SmcPagedSeqs
+{
+    public nint Table, Lengths, RowStart;   // RowStart may be 0: one row per sequence
+    public int Batch, Width, Rows;
+}
+
 internal static unsafe partial class Native
 {
     const string Lib = "sharpmind_cuda";   // libsharpmind_cuda.so next to the assembly
@@ -138,6 +155,14 @@ internal static unsafe partial class Native
     [LibraryImport(Lib)] internal static partial int smc_kv_restore(nint ctx, nint kv, void* hostK, void* hostV, long bytesEach, int position);
     [LibraryImport(Lib)] internal static partial int smc_sdpa_kv_dev(nint ctx, nint kv, nint dQ, nint dOut, int batch, int heads, int seqLen,
         float scale, nint stream);
+
+    // ---- paged cache
+    [LibraryImport(Lib)] internal static partial int smc_paged_update_dev(nint ctx, in SmcPagedKv kv, in SmcPagedSeqs seqs, int dtype, nint dK, long kStride,
+        nint dV, long vStride, nint dQ, long qStride, nint dQOut, int heads, nint dCos, nint dSin, int ropeDim, int tableRows, int neox, nint stream);
+    [LibraryImport(Lib)] internal static partial int smc_paged_read_dev(nint ctx, in SmcPagedKv kv, nint dPages, int n, int dtype, nint dK, nint dV, nint stream);
+    [LibraryImport(Lib)] internal static partial long smc_paged_attention_work(nint ctx, in SmcPagedKv kv, int batch, int heads, int maxRows, int maxLen);
+    [LibraryImport(Lib)] internal static partial int smc_paged_attention_dev(nint ctx, in SmcPagedKv kv, in SmcPagedSeqs seqs, int dtype, nint dQ, long qStride,
+        nint dOut, int heads, float scale, int window, int maxRows, int maxLen, nint dWork, long workBytes, nint stream);
 
     // ---- resident decoder
     [LibraryImport(Lib)] internal static partial int smc_model_create(nint ctx, in SmcModelDesc desc, int maxBatch, out nint model);
