@@ -309,7 +309,8 @@ int64_t smc_paged_attention_work(smc_ctx *ctx, const smc_paged_kv *kv, int batch
 {
     if (check_cache(ctx, "paged_attention_work", kv, SMC_F32)) return -1;
     if (batch < 0 || heads <= 0 || heads % kv->kv_heads || max_rows < 0 || max_len < 0) return smc_fail(ctx, -1, "paged_attention_work: bad arguments");
-    return 0;
+    // (the most of both types of activations)
+    return smc_paged_decode_takes(1, heads / kv->kv_heads, max_rows) ? (int64_t)smc_paged_decode_work(ctx, kv->kv_heads, batch, heads, kv->head_dim, max_rows, max_len) : 0;
 }
 
 int smc_paged_attention_dev(smc_ctx *ctx, const smc_paged_kv *kv, const smc_paged_seqs *seqs, int dtype, const void *d_q, long long q_stride, void *d_out, int heads,
@@ -322,8 +323,16 @@ int smc_paged_attention_dev(smc_ctx *ctx, const smc_paged_kv *kv, const smc_page
     if (seqs->rows == 0 || seqs->batch == 0) return SMC_OK;
     if (bad_rows(d_q, q_stride, heads, kv->head_dim, dtype) || !d_out || !aligned(d_out))
         return smc_fail(ctx, SMC_E_INVALID, "paged_attention: rows must start on 16-byte boundaries and hold their heads");
-    (void)d_work, (void)work_bytes;
+    if ((long long)seqs->batch * kv->kv_heads * ((long long)seqs->width * kv->page / 64 + 1) > 0x7FFFFFFF)
+        return smc_fail(ctx, SMC_E_UNSUPPORTED, "paged_attention: a table of %d x %d pages of %d heads", seqs->batch, seqs->width, kv->kv_heads);
     OnDevice on(ctx->device);
     const smc_paged_query q{d_q, q_stride, d_out, dtype == SMC_BF16, heads, kv->head_dim, window, max_rows, max_len, scale};
-    return smc_launch_paged_attend(ctx, view(kv, seqs), q, static_cast<cudaStream_t>(stream));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (smc_paged_decode_takes(q.bf16, heads / kv->kv_heads, max_rows)) {
+        if (max_rows == 0) return smc_fail(ctx, SMC_E_INVALID, "paged_attention: %d rows, none of a sequence", seqs->rows);
+        if (!d_work || !aligned(d_work) || work_bytes < smc_paged_attention_work(ctx, kv, seqs->batch, heads, max_rows, max_len))
+            return smc_fail(ctx, SMC_E_INVALID, "paged_attention: %lld bytes of work space are not enough, or not on a 16-byte boundary", work_bytes);
+        return smc_launch_paged_decode(ctx, view(kv, seqs), q, static_cast<float *>(d_work), s);
+    }
+    return smc_launch_paged_attend(ctx, view(kv, seqs), q, s);
 }
