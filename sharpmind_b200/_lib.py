@@ -82,7 +82,7 @@ SIGNATURES = {
     "smc_paged_update_dev": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int,
                                      c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
     "smc_paged_read_dev": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p]),
-    "smc_paged_attention_work": (c_int64, [c_void_p, c_void_p, c_int, c_int, c_int, c_int]),
+    "smc_paged_attention_work": (c_int64, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int]),
     "smc_paged_attention_dev": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int, c_float, c_int, c_int, c_int,
                                         c_void_p, c_int64, c_void_p]),
     "smc_model_create": (c_int, [c_void_p, c_void_p, c_int, _pp]),

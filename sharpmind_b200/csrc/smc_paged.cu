@@ -1,5 +1,5 @@
 // The paged key/value cache: entry points, the update that rotates, quantises and places new tokens, and the read that turns pages back into
-// values.  The attention over it: smc_paged_attend.cu.
+// values.  The attention over it: smc_paged_decode.cu, smc_paged_prompt.cu.
 //
 // A block is the tokens of one page and head, keys and values apart.  Its scale is 2^k, k = min{k >= -40 : amax <= 448 2^k}, amax over all that
 // entered the block since its first token; a value is held as code = e4m3(x / scale) and stands for code * scale.  Dividing by a power of two is exact, so
@@ -305,12 +305,16 @@ int smc_paged_read_dev(smc_ctx *ctx, const smc_paged_kv *kv, const int *d_pages,
     return SMC_OK;
 }
 
-int64_t smc_paged_attention_work(smc_ctx *ctx, const smc_paged_kv *kv, int batch, int heads, int max_rows, int max_len)
+int64_t smc_paged_attention_work(smc_ctx *ctx, const smc_paged_kv *kv, int batch, int rows, int heads, int max_rows, int max_len)
 {
     if (check_cache(ctx, "paged_attention_work", kv, SMC_F32)) return -1;
-    if (batch < 0 || heads <= 0 || heads % kv->kv_heads || max_rows < 0 || max_len < 0) return smc_fail(ctx, -1, "paged_attention_work: bad arguments");
-    // (the most of both types of activations)
-    return smc_paged_decode_takes(1, heads / kv->kv_heads, max_rows) ? (int64_t)smc_paged_decode_work(ctx, kv->kv_heads, batch, heads, kv->head_dim, max_rows, max_len) : 0;
+    if (batch < 0 || rows < 0 || heads <= 0 || heads % kv->kv_heads || max_rows < 0 || max_len < 0) return smc_fail(ctx, -1, "paged_attention_work: bad arguments");
+    // (the type of the activations is not known here: the form may be either)
+    const int group = heads / kv->kv_heads;
+    size_t n = 0;
+    if (smc_paged_decode_takes(1, group, max_rows)) n = smc_paged_decode_work(ctx, kv->kv_heads, batch, heads, kv->head_dim, max_rows, max_len);
+    if (!smc_paged_decode_takes(0, group, max_rows)) n = std::max(n, smc_paged_prompt_work(ctx, kv->kv_heads, batch, rows, heads, kv->head_dim, max_len));
+    return (int64_t)n;
 }
 
 int smc_paged_attention_dev(smc_ctx *ctx, const smc_paged_kv *kv, const smc_paged_seqs *seqs, int dtype, const void *d_q, long long q_stride, void *d_out, int heads,
@@ -328,11 +332,10 @@ int smc_paged_attention_dev(smc_ctx *ctx, const smc_paged_kv *kv, const smc_page
     OnDevice on(ctx->device);
     const smc_paged_query q{d_q, q_stride, d_out, dtype == SMC_BF16, heads, kv->head_dim, window, max_rows, max_len, scale};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (smc_paged_decode_takes(q.bf16, heads / kv->kv_heads, max_rows)) {
-        if (max_rows == 0) return smc_fail(ctx, SMC_E_INVALID, "paged_attention: %d rows, none of a sequence", seqs->rows);
-        if (!d_work || !aligned(d_work) || work_bytes < smc_paged_attention_work(ctx, kv, seqs->batch, heads, max_rows, max_len))
-            return smc_fail(ctx, SMC_E_INVALID, "paged_attention: %lld bytes of work space are not enough, or not on a 16-byte boundary", work_bytes);
-        return smc_launch_paged_decode(ctx, view(kv, seqs), q, static_cast<float *>(d_work), s);
-    }
-    return smc_launch_paged_attend(ctx, view(kv, seqs), q, s);
+    if (max_rows == 0) return smc_fail(ctx, SMC_E_INVALID, "paged_attention: %d rows, none of a sequence", seqs->rows);
+    const int64_t need = smc_paged_attention_work(ctx, kv, seqs->batch, seqs->rows, heads, max_rows, max_len);
+    if (need > 0 && (!d_work || !aligned(d_work) || work_bytes < need))
+        return smc_fail(ctx, SMC_E_INVALID, "paged_attention: %lld bytes of work space are not enough, or not on a 16-byte boundary", work_bytes);
+    if (smc_paged_decode_takes(q.bf16, heads / kv->kv_heads, max_rows)) return smc_launch_paged_decode(ctx, view(kv, seqs), q, static_cast<float *>(d_work), s);
+    return smc_launch_paged_prompt(ctx, view(kv, seqs), q, static_cast<float *>(d_work), s);
 }

@@ -80,7 +80,7 @@ template <typename T> __device__ __forceinline__ void smc_paged_load4(const T *p
 template <typename T> __device__ __forceinline__ void smc_paged_store4(T *p, const float (&f)[4]) { store_v<T, 4>(p, f); }
 #endif
 
-// Launchers of the attention's forms: a few rows of every sequence (smc_paged_decode.cu), and any (smc_paged_attend.cu)
+// Launchers of the attention's forms: a few rows of every sequence (smc_paged_decode.cu), or many (smc_paged_prompt.cu)
 struct smc_paged_query {
     const void *q;
     long long q_stride;
@@ -91,4 +91,5 @@ struct smc_paged_query {
 bool smc_paged_decode_takes(int bf16, int group, int max_rows);
 size_t smc_paged_decode_work(const smc_ctx *, int kvh, int batch, int heads, int hd, int max_rows, int max_len);
 int smc_launch_paged_decode(smc_ctx *, const smc_paged_view &, const smc_paged_query &, float *work, cudaStream_t s);
-int smc_launch_paged_attend(smc_ctx *, const smc_paged_view &, const smc_paged_query &, cudaStream_t s);
+size_t smc_paged_prompt_work(const smc_ctx *, int kvh, int batch, int rows, int heads, int hd, int max_len);
+int smc_launch_paged_prompt(smc_ctx *, const smc_paged_view &, const smc_paged_query &, float *work, cudaStream_t s);

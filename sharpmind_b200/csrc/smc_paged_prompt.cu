@@ -1,0 +1,531 @@
+// Attention of many rows over the paged cache (a prompt, a chunk of one, long drafts) on the fifth-generation tensor cores.
+//
+// One CTA = up to 256 (row, query head) pairs of one sequence and KV head, two tiles of 128, a thread a pair; keys in tiles of KT.  The codes are brought as
+// they lie in their pages, turned to fp16 (exact) by four warps and stored as 128-byte-swizzled K-major tiles, once for all heads of a group and both
+// tiles.  Scores S = Q K^T and outputs O += P V are tcgen05.mma, fp16 with fp32 sums in tensor memory, P in the columns that S leaves:
+//   bfloat16  queries exact in fp16 after a power of two per row, weights rounded to 11 bits; KT = 128
+//   fp32      queries and weights as hi + lo, 22 bits, two products each; KT = 64
+// With the pages' scales, constant over 16 keys:  y = S f + b, f = s_k * row factor, b = log2(s_v);  w = 2^(y - R);  l = sum w / s_v;  out = O / l.
+// R follows the running maximum of y only where that gets more than 2^15 above it (then to 2^8 below), so O, in tensor memory, is rarely
+// multiplied again; a weight stays under 2^15 and counts down to 2^-24.
+// Warp roles:  0 .. 3, 4 .. 7  softmax of tile 0, 1      8 .. 11  codes to fp16      12  MMA issue
+// MMA order per key tile i:  O0 += P0(i) V(i), S0(i + 1), O1 += P1(i) V(i), S1(i + 1): one tile's products run under the other's softmax.  MMAs of one
+// thread run in order, so S(i + 1) may overwrite P(i), and a softmax that has S(i + 1) may touch O.
+// Few pairs: the key tiles are split over CTAs, whose partial results a second kernel joins.
+#include "smc_paged.cuh"
+#include "smc_tc.cuh"
+
+namespace {
+
+constexpr int PAIRS = 256, TILE = 128, SOFT_WARPS = 8, CONV_WARP = 8, MMA_WARP = 12, THREADS = 512, SC_SLOTS = 4;
+constexpr float R_ABOVE = 15.0f, R_BELOW = 8.0f;
+
+template <int HD, bool SPLIT>
+struct Shape {
+    static constexpr int PLANES = SPLIT ? 2 : 1, KT = SPLIT ? 64 : 128;
+    static constexpr uint32_t SUB_Q = TILE * 128, Q_PLANE = HD / 64 * SUB_Q, Q_TILE = PLANES * Q_PLANE;
+    static constexpr uint32_t STAGE = KT * HD * 2;  // fp16 keys or values of a tile
+    static constexpr uint32_t OFF_K = 2 * Q_TILE, OFF_V = OFF_K + 2 * STAGE, OFF_SC = OFF_V + 2 * STAGE, OFF_BAR = OFF_SC + SC_SLOTS * (KT / 16) * 16, SMEM = OFF_BAR + 256;
+    static constexpr uint32_t COL_S = 0, COL_O = 256, COLS = 512;
+    static_assert(SMEM <= 227 * 1024 && COL_O + 2 * HD <= COLS && 2 * KT <= COL_O, "");
+};
+enum { K_FULL = 0, K_EMPTY = 2, V_FULL = 4, V_EMPTY = 6, S_FULL = 8, P_FULL = 10, O_FULL = 12, Q_FULL = 14, BARS = 16 };
+
+__device__ __forceinline__ void mma_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)  // A in tensor memory
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r)
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+        "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w)
+{
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ uint32_t half2_bits(float a, float b)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t rest_bits(float a, float b, uint32_t hi)
+{
+    const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+    return half2_bits(a - h.x, b - h.y);
+}
+__host__ __device__ constexpr uint32_t idesc_f16(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TILE >> 4) << 24); }
+
+// What a CTA does: pairs [m0, m0 + pairs) of sequence s and head h; key tiles [kv0, kv0 + n[t]) of tile t, of which this piece takes [i0, i1).
+struct Job {
+    int s, h, m0, pairs, len, n_rows, r0, from, kv0, n0, n1, i0, i1, piece, pieces;
+};
+template <int KT>
+__device__ __forceinline__ bool job_of(const smc_paged_view &c, const smc_paged_query &u, int item, int h, int piece, int split, Job &j, int *status)
+{
+    const int group = u.heads / c.kvh;
+    auto items_before = [&](int s) { return (int)((long long)min(max(c.row_start ? c.row_start[s] : s, 0), c.rows) * group / PAIRS) + s; };
+    int lo = 0, hi = c.batch;  // the last sequence whose items start at or before this one
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (items_before(mid) <= item) lo = mid;
+        else hi = mid;
+    }
+    const smc_paged_seq sq = smc_paged_sequence(c, lo);
+    if ((sq.bad || sq.n > u.max_rows) && status) *status = SMC_STATUS_PAGED;
+    const int local = item - items_before(lo);
+    const long long all = (long long)sq.n * group;
+    if (local < 0 || (long long)local * PAIRS >= all) return false;
+    j.s = lo, j.h = h, j.m0 = local * PAIRS, j.pairs = (int)min((long long)PAIRS, all - j.m0);
+    j.len = sq.len, j.n_rows = sq.n, j.r0 = sq.r0;
+    const int p0 = sq.len - sq.n;  // position of the sequence's first row
+    const int first = p0 + j.m0 / group, end0 = p0 + (j.m0 + min(j.pairs, TILE) - 1) / group + 1, end1 = p0 + (j.m0 + j.pairs - 1) / group + 1;
+    j.from = u.window > 0 ? max(0, first - u.window + 1) : 0;
+    j.kv0 = j.from / KT;
+    j.n0 = max(1, (end0 + KT - 1) / KT - j.kv0), j.n1 = j.pairs > TILE ? max(j.n0, (end1 + KT - 1) / KT - j.kv0) : j.n0;
+    j.pieces = min(split, j.n1), j.piece = piece;
+    if (piece >= j.pieces) return false;
+    j.i0 = (int)((long long)piece * j.n1 / j.pieces), j.i1 = (int)((long long)(piece + 1) * j.n1 / j.pieces);
+    return true;
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_paged_view c, const smc_paged_query u, int items, int split, float *work, int *status)
+{
+    constexpr bool SPLIT = sizeof(T) == 4;
+    using S = Shape<HD, SPLIT>;
+    constexpr int KT = S::KT, G = KT / 16;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const uint32_t sbase = smc_smem_u32(smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem + S::OFF_BAR + BARS * 8 + 4);
+    auto bar = [&](int i) { return sbase + S::OFF_BAR + 8u * (uint32_t)i; };
+    auto wait = [&](int i, uint32_t parity) {  // by whole warps: one lane polls
+        if (lane == 0) smc_tc_wait(bar(i), parity & 1u, abort_flag, status);
+        __syncwarp();
+    };
+    auto arrive = [&](int i) {
+        __syncwarp();
+        if (lane == 0) smc_mbar_arrive(bar(i));
+    };
+    // tensor memory is taken after the predecessor has completed and before the successor may start
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    Job j;
+    {
+        int b = blockIdx.x;
+        const int piece = b % split;
+        b /= split;
+        const int h = b % c.kvh, item = items - 1 - b / c.kvh;  // later rows see more keys: they start first
+        if (!job_of<KT>(c, u, item, h, piece, split, j, threadIdx.x == 0 ? status : nullptr)) {  // (the same for all threads)
+            asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+            return;
+        }
+    }
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            smc_mbar_init(bar(K_FULL + i), 4), smc_mbar_init(bar(K_EMPTY + i), 1), smc_mbar_init(bar(V_FULL + i), 4), smc_mbar_init(bar(V_EMPTY + i), 1);
+            smc_mbar_init(bar(S_FULL + i), 1), smc_mbar_init(bar(P_FULL + i), 4), smc_mbar_init(bar(O_FULL + i), 1), smc_mbar_init(bar(Q_FULL + i), 4);
+        }
+        *abort_flag = 0;
+        smc_fence_barrier_init();
+    }
+    if (warp == MMA_WARP) {
+        __syncwarp();
+        smc_tc_alloc(sbase + S::OFF_BAR + BARS * 8, S::COLS);
+    }
+    smc_tc_fence_before();
+    __syncthreads();
+    smc_tc_fence_after();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + S::OFF_BAR + BARS * 8);
+    const int group = u.heads / c.kvh;
+    const bool two = j.pairs > TILE;
+    const int stop0 = min(j.n0, j.i1), stop1 = two ? j.i1 : j.i0;  // tile t takes [i0, stop)
+
+    if (warp < SOFT_WARPS) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+        const int t = warp >> 2, rl = 32 * (warp & 3) + lane, m = t * TILE + rl, stop = t ? stop1 : stop0;
+        const bool real = m < j.pairs;
+        const int pair = j.m0 + (real ? m : 0), tok = pair / group, head = j.h * group + pair - tok * group;
+        const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16), col_s = lanes + S::COL_S + (uint32_t)(t * KT), col_o = lanes + S::COL_O + (uint32_t)(t * HD);
+        const int pos = j.len - j.n_rows + tok;
+        float rowf = 0.0f, R = -INFINITY, l = 0.0f;
+        if (stop > j.i0) {
+            const T *src = static_cast<const T *>(u.q) + (long long)(j.r0 + tok) * u.q_stride + (size_t)head * HD;
+            float most = 0.0f;
+#pragma unroll 8
+            for (int e = 0; e < HD; e += 4) {
+                float v[4];
+                smc_paged_load4(src + e, v);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) most = fmaxf(most, fabsf(v[k]));
+            }
+            // the largest magnitude of the row goes to [2^14, 2^15); a negative scale turns the queries' sign
+            const int up = min(14 - ((int)(__float_as_uint(most) >> 23) - 127), 126);
+            float fac = __uint_as_float((uint32_t)(up + 127) << 23);
+            rowf = fabsf(u.scale) * 1.44269504088896341f * __uint_as_float((uint32_t)(127 - up) << 23);
+            if (u.scale < 0.0f) fac = -fac;
+            if (!real) fac = 0.0f;
+#pragma unroll 4
+            for (int e = 0; e < HD; e += 8) {
+                float v[8], a[4], b[4];
+                smc_paged_load4(src + e, a), smc_paged_load4(src + e + 4, b);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = a[k] * fac, v[4 + k] = b[k] * fac;
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    hi[k] = half2_bits(v[2 * k], v[2 * k + 1]);
+                    if (SPLIT) lo[k] = rest_bits(v[2 * k], v[2 * k + 1], hi[k]);
+                }
+                const uint32_t at = sbase + (uint32_t)t * S::Q_TILE + (uint32_t)(e >> 6) * S::SUB_Q + (uint32_t)(rl >> 3) * 1024u + (uint32_t)(rl & 7) * 128u +
+                                    (uint32_t)((((e >> 3) & 7) ^ (rl & 7)) << 4);
+                sts128(at, hi[0], hi[1], hi[2], hi[3]);
+                if (SPLIT) sts128(at + S::Q_PLANE, lo[0], lo[1], lo[2], lo[3]);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            arrive(Q_FULL + t);
+        }
+        // rows of this tile: [lowest, highest] positions, for tiles that every row sees whole
+        const int lowest = j.len - j.n_rows + (j.m0 + t * TILE) / group, highest = j.len - j.n_rows + (j.m0 + min(j.pairs, (t + 1) * TILE) - 1) / group;
+#pragma unroll 1
+        for (int i = j.i0; i < stop; ++i) {
+            const int it = i - j.i0, key0 = (j.kv0 + i) * KT;
+            wait(S_FULL + t, (uint32_t)it);
+            smc_tc_fence_after();
+            uint32_t s[KT];
+#pragma unroll
+            for (int k = 0; k < KT; k += 16) smc_tc_ld16(col_s + (uint32_t)k, *reinterpret_cast<uint32_t(*)[16]>(s + k));
+            const float4 *sc = reinterpret_cast<const float4 *>(smem + S::OFF_SC) + (it % SC_SLOTS) * G;
+            smc_tc_wait_ld();
+            const bool inner = key0 + KT <= lowest + 1 && (u.window <= 0 || key0 > highest - u.window);
+            if (!inner) {
+                const int hi = pos - key0, lo = u.window > 0 ? hi - u.window : -1;
+#pragma unroll
+                for (int k = 0; k < KT; ++k)
+                    if (k > hi || k <= lo) s[k] = 0xFF800000u;  // -infinity
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < G; ++k) {
+                const float4 x = sc[k];
+                float gm = __uint_as_float(s[16 * k]);
+#pragma unroll
+                for (int e = 1; e < 16; ++e) gm = fmaxf(gm, __uint_as_float(s[16 * k + e]));
+                top = fmaxf(top, fmaf(gm, x.x * rowf, x.y));  // (hidden keys, -inf, times 0 or an undefined scale: not a number, which a maximum drops)
+            }
+            float corr = 1.0f;
+            if (top > R + R_ABOVE) {
+                const float was = R;
+                R = top - R_BELOW;
+                corr = ex2(was - R);
+            }
+            if (__any_sync(0xFFFFFFFFu, corr != 1.0f)) {
+                l *= corr;
+                if (it > 0) {
+#pragma unroll 1
+                    for (int k = 0; k < HD; k += 16) {
+                        uint32_t o[16];
+                        smc_tc_ld16(col_o + (uint32_t)k, o);
+                        smc_tc_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+                        tmem_st16(col_o + (uint32_t)k, o);
+                    }
+                }
+            }
+            const float ref = R == -INFINITY ? 0.0f : R;
+            uint32_t rest[SPLIT ? KT / 2 : 1];
+#pragma unroll
+            for (int k = 0; k < G; ++k) {
+                const float4 x = sc[k];
+                const float f = x.x * rowf, b = x.y - ref;
+                float w[16], sum = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) w[e] = ex2(fmaf(__uint_as_float(s[16 * k + e]), f, b));
+                if (!inner) {
+                    const int hi = pos - key0 - 16 * k, lo = u.window > 0 ? hi - u.window : -1;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (e > hi || e <= lo) w[e] = 0.0f;
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sum += w[e];
+                // (a row that sees none of these keys takes nothing of their scale, which may be undefined)
+                l = inner ? fmaf(sum, x.z, l) : l + (sum == 0.0f ? 0.0f : sum * x.z);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t hi = half2_bits(w[2 * e], w[2 * e + 1]);
+                    if constexpr (SPLIT) rest[8 * k + e] = rest_bits(w[2 * e], w[2 * e + 1], hi);
+                    s[8 * k + e] = hi;  // (the scores there are used up)
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < KT / 2; k += 16) {
+                tmem_st16(col_s + (uint32_t)k, s + k);
+                if constexpr (SPLIT) tmem_st16(col_s + (uint32_t)(KT / 2 + k), rest + k);
+            }
+            tmem_wait_st();
+            smc_tc_fence_before();
+            arrive(P_FULL + t);
+        }
+        if (stop > j.i0) {
+            wait(O_FULL + t, 0);
+            smc_tc_fence_after();
+            const float norm = j.pieces > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+            T *dst = static_cast<T *>(u.out) + ((size_t)(j.r0 + tok) * u.heads + head) * HD;
+            float *part = work + ((size_t)blockIdx.x * PAIRS + m) * (HD + 4);
+#pragma unroll 1
+            for (int k = 0; k < HD; k += 16) {
+                uint32_t o[16];
+                smc_tc_ld16(col_o + (uint32_t)k, o);
+                smc_tc_wait_ld();
+                if (real) {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        const float v[4] = {__uint_as_float(o[e]) * norm, __uint_as_float(o[e + 1]) * norm, __uint_as_float(o[e + 2]) * norm, __uint_as_float(o[e + 3]) * norm};
+                        if (j.pieces > 1) smc_paged_store4(part + k + e, v);
+                        else smc_paged_store4(dst + k + e, v);
+                    }
+                }
+                __syncwarp();
+            }
+            if (real && j.pieces > 1) part[HD] = R, part[HD + 1] = l;
+        } else if (real && j.pieces > 1) {  // a piece behind the last key that this tile sees
+            float *part = work + ((size_t)blockIdx.x * PAIRS + m) * (HD + 4);
+            const float zero[4] = {};
+            for (int k = 0; k < HD; k += 4) smc_paged_store4(part + k, zero);
+            part[HD] = -INFINITY, part[HD + 1] = 0.0f;
+        }
+    } else if (warp < MMA_WARP) {
+        // ---------------------------------------------------------------- codes to fp16
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        const int w = warp - CONV_WARP, page = 1 << c.shift;
+        constexpr int UNITS = KT * HD / 16 / 128;  // 16 codes a thread each
+        const int hi = min(j.len, j.len - j.n_rows + (j.m0 + j.pairs - 1) / group + 1);  // keys [from, hi) count
+        // page of this lane's group of 16 keys (lane % G) of tile i, or -1
+        auto page_of = [&](int i) {
+            const int key = (j.kv0 + i) * KT + 16 * (lane % G), p0 = key >> c.shift << c.shift;
+            if (i >= j.i1 || p0 + page <= j.from || p0 >= hi) return -1;  // (pages that left the window may have gone to another sequence)
+            const int id = smc_paged_page(c, j.s, key >> c.shift);
+            if (id < 0) *status = SMC_STATUS_PAGED;
+            return id;
+        };
+        const int r8 = lane & 7, q4 = lane >> 3;
+        auto fetch = [&](const uint8_t *base, int ids, bool values, int i, int x) {
+            const int inner = values ? KT / 64 : HD / 64, big = x / inner, half = x - big * inner;
+            const int group16 = values ? 4 * half + q4 : big >> 1;  // of the tile's keys
+            const int id = __shfl_sync(0xFFFFFFFFu, ids, group16);
+            uint4 v = make_uint4(0, 0, 0, 0);
+            const int key = (j.kv0 + i) * KT + (values ? 16 * group16 : 8 * big + r8);
+            if (id >= 0) {
+                const uint8_t *p = base + ((size_t)id * c.kvh + j.h) * ((size_t)HD << c.shift);
+                p += values ? ((8 * big + r8) << c.shift) + (key & (page - 1)) : (key & (page - 1)) * HD + 64 * half + 16 * q4;
+                v = __ldcg(reinterpret_cast<const uint4 *>(p));
+                if (values) {  // values that do not count are zeros whatever their bytes are: the weights there are 0, and codes may be undefined
+                    if (key < j.from || key + 16 > hi) {
+                        uint32_t *b = &v.x;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (key + e < j.from || key + e >= hi) b[e >> 2] &= ~(0xFFu << (8 * (e & 3)));
+                    }
+                } else if (key >= hi) {
+                    v = make_uint4(0, 0, 0, 0);
+                }
+            }
+            return v;
+        };
+        auto place = [&](uint32_t stage, bool values, int x, const uint4 &v) {
+            const int inner = values ? KT / 64 : HD / 64, big = x / inner, half = x - big * inner;
+            const uint32_t row = stage + (uint32_t)half * (uint32_t)((values ? HD : KT) * 128) + (uint32_t)big * 1024u + (uint32_t)r8 * 128u;
+            const uint32_t raw[4] = {v.x, v.y, v.z, v.w};
+            uint32_t h[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) h[2 * e] = smc_e4m3x2_half2(raw[e] & 0xFFFFu), h[2 * e + 1] = smc_e4m3x2_half2(raw[e] >> 16);
+            sts128(row + (uint32_t)(((2 * q4) ^ r8) << 4), h[0], h[1], h[2], h[3]);
+            sts128(row + (uint32_t)(((2 * q4 + 1) ^ r8) << 4), h[4], h[5], h[6], h[7]);
+        };
+        auto scales = [&](int i, int ids) {
+            if (w == 0 && lane < G) {
+                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (ids >= 0) {
+                    const float2 s2 = *reinterpret_cast<const float2 *>(c.scales + 2 * ((size_t)ids * c.kvh + j.h));
+                    // (a power of two's exponent; an undefined scale stays what it is)
+                    x = make_float4(s2.x, s2.y == s2.y ? (float)((int)(__float_as_uint(s2.y) >> 23) - 127) : s2.y, 1.0f / s2.y, 0.0f);
+                }
+                reinterpret_cast<float4 *>(smem + S::OFF_SC)[((i - j.i0) % SC_SLOTS) * G + lane] = x;
+            }
+        };
+        uint4 raw[UNITS];
+        int ids = page_of(j.i0), ids_next = page_of(j.i0 + 1);
+#pragma unroll
+        for (int x = 0; x < UNITS; ++x) raw[x] = fetch(c.k, ids, false, j.i0, w + 4 * x);
+#pragma unroll 1
+        for (int i = j.i0; i < j.i1; ++i) {
+            const int it = i - j.i0, st = it & 1;
+            const uint32_t parity = (uint32_t)(it >> 1) ^ 1u;  // (a fresh barrier passes the first)
+            wait(K_EMPTY + st, parity);
+            scales(i, ids);
+#pragma unroll
+            for (int x = 0; x < UNITS; ++x) {  // as a unit's registers are free, they take the codes of the next half
+                place(sbase + S::OFF_K + (uint32_t)st * S::STAGE, false, w + 4 * x, raw[x]);
+                raw[x] = fetch(c.v, ids, true, i, w + 4 * x);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            arrive(K_FULL + st);
+            const int after = page_of(i + 2);
+            wait(V_EMPTY + st, parity);
+#pragma unroll
+            for (int x = 0; x < UNITS; ++x) {
+                place(sbase + S::OFF_V + (uint32_t)st * S::STAGE, true, w + 4 * x, raw[x]);
+                raw[x] = fetch(c.k, ids_next, false, i + 1, w + 4 * x);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            arrive(V_FULL + st);
+            ids = ids_next, ids_next = after;
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        if (warp == MMA_WARP && lane == 0) {
+            // ---------------------------------------------------------------- MMA issue
+            auto scores = [&](int t, int it) {
+                const int st = it & 1;
+                const uint32_t d = tmem + S::COL_S + (uint32_t)(t * KT);
+                const uint64_t k0 = smc_tc_desc_sw128(sbase + S::OFF_K + (uint32_t)st * S::STAGE), q0 = smc_tc_desc_sw128(sbase + (uint32_t)t * S::Q_TILE);
+#pragma unroll
+                for (int p = S::PLANES - 1; p >= 0; --p)  // smallest products first
+#pragma unroll
+                    for (int ks = 0; ks < HD / 16; ++ks)
+                        smc_tc_mma(d, q0 + (uint64_t)(((uint32_t)p * S::Q_PLANE + (uint32_t)(ks >> 2) * S::SUB_Q + (uint32_t)(ks & 3) * 32u) >> 4),
+                                   k0 + (uint64_t)(((uint32_t)(ks >> 2) * (uint32_t)(KT * 128) + (uint32_t)(ks & 3) * 32u) >> 4), idesc_f16(KT), p < S::PLANES - 1 || ks > 0);
+                smc_tc_commit(bar(S_FULL + t));
+            };
+            auto outputs = [&](int t, int it) {
+                const int st = it & 1;
+                const uint32_t d = tmem + S::COL_O + (uint32_t)(t * HD), a = tmem + S::COL_S + (uint32_t)(t * KT);
+                const uint64_t v0 = smc_tc_desc_sw128(sbase + S::OFF_V + (uint32_t)st * S::STAGE);
+#pragma unroll
+                for (int p = S::PLANES - 1; p >= 0; --p)
+#pragma unroll
+                    for (int kk = 0; kk < KT / 16; ++kk)
+                        mma_ta(d, a + (uint32_t)(p * KT / 2 + kk * 8), v0 + (uint64_t)(((uint32_t)(kk >> 2) * (uint32_t)(HD * 128) + (uint32_t)(kk & 3) * 32u) >> 4), idesc_f16(HD),
+                               it > 0 || p < S::PLANES - 1 || kk > 0);
+            };
+            const int n0 = stop0 - j.i0, n1 = stop1 - j.i0, n = j.i1 - j.i0;  // (n0 <= n; n1 is n or 0)
+            smc_tc_wait(bar(K_FULL), 0u, abort_flag, status);
+            if (n0 > 0) {
+                smc_tc_wait(bar(Q_FULL), 0u, abort_flag, status);
+                smc_tc_fence_after();
+                scores(0, 0);
+            }
+            if (n1 > 0) {
+                smc_tc_wait(bar(Q_FULL + 1), 0u, abort_flag, status);
+                smc_tc_fence_after();
+                scores(1, 0);
+            }
+            smc_tc_commit(bar(K_EMPTY));
+#pragma unroll 1
+            for (int it = 0; it < n; ++it) {
+                const int st = it & 1, nx = (it + 1) & 1;
+                smc_tc_wait(bar(V_FULL + st), (uint32_t)(it >> 1) & 1u, abort_flag, status);
+                if (it < n0) {
+                    smc_tc_wait(bar(P_FULL), (uint32_t)it & 1u, abort_flag, status);
+                    smc_tc_fence_after();
+                    outputs(0, it);
+                    if (it + 1 == n0) smc_tc_commit(bar(O_FULL));
+                }
+                if (it + 1 < n) {
+                    smc_tc_wait(bar(K_FULL + nx), (uint32_t)((it + 1) >> 1) & 1u, abort_flag, status);
+                    smc_tc_fence_after();
+                    if (it + 1 < n0) scores(0, it + 1);
+                }
+                if (it < n1) {
+                    smc_tc_wait(bar(P_FULL + 1), (uint32_t)it & 1u, abort_flag, status);
+                    smc_tc_fence_after();
+                    outputs(1, it);
+                    if (it + 1 == n1) smc_tc_commit(bar(O_FULL + 1));
+                    if (it + 1 < n1) scores(1, it + 1);
+                }
+                smc_tc_commit(bar(V_EMPTY + st));
+                if (it + 1 < n) smc_tc_commit(bar(K_EMPTY + nx));
+            }
+        }
+        __syncwarp();
+    }
+    smc_tc_fence_before();
+    __syncthreads();
+    if (warp == MMA_WARP) {
+        __syncwarp();
+        smc_tc_dealloc(tmem, S::COLS);
+    }
+}
+
+// One warp = one pair of a job whose keys were split: joins the pieces in their order.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) paged_prompt_join_kernel(const smc_paged_view c, const smc_paged_query u, int items, int split, const float *__restrict__ work)
+{
+    smc_grid_dep_sync();
+    constexpr int KT = Shape<HD, sizeof(T) == 4>::KT, E = HD / 32;
+    const int lane = threadIdx.x & 31, b = blockIdx.x / (PAIRS / 8), m = blockIdx.x % (PAIRS / 8) * 8 + (threadIdx.x >> 5);
+    Job j;
+    if (!job_of<KT>(c, u, items - 1 - b / c.kvh, b % c.kvh, 0, split, j, nullptr) || j.pieces == 1 || m >= j.pairs) return;
+    const float *row = work + ((size_t)b * split * PAIRS + m) * (HD + 4);
+    const size_t step = (size_t)PAIRS * (HD + 4);
+    float top = -INFINITY, sum = 0.0f, o[E] = {};
+    for (int i = 0; i < j.pieces; ++i) top = fmaxf(top, row[i * step + HD]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    for (int i = 0; i < j.pieces; ++i) {
+        const float f = ex2(row[i * step + HD] - ref);
+        sum = fmaf(row[i * step + HD + 1], f, sum);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = fmaf(row[i * step + lane + 32 * e], f, o[e]);
+    }
+    const int group = u.heads / c.kvh, pair = j.m0 + m, tok = pair / group;
+    T *dst = static_cast<T *>(u.out) + ((size_t)(j.r0 + tok) * u.heads + j.h * group + pair - tok * group) * HD;
+#pragma unroll
+    for (int e = 0; e < E; ++e) dst[lane + 32 * e] = from_f<T>(sum == 0.0f ? 0.0f : o[e] / sum);
+}
+
+// jobs of a call (some may be empty: a sequence's share is rounded up), and into how many pieces each one's keys go
+long long items_of(int batch, int rows, int group) { return (long long)rows * group / PAIRS + batch; }
+int split_of(const smc_ctx *ctx, int kvh, int batch, int rows, int group, int max_len)
+{
+    const long long jobs = items_of(batch, rows, group) * kvh;
+    return (int)std::max(1LL, std::min((long long)max_len / 256, (long long)ctx->sm_count / std::max(1LL, jobs)));
+}
+
+}  // namespace
+
+size_t smc_paged_prompt_work(const smc_ctx *ctx, int kvh, int batch, int rows, int heads, int hd, int max_len)
+{
+    const int split = split_of(ctx, kvh, batch, rows, heads / kvh, max_len);
+    return split == 1 ? 0 : (size_t)items_of(batch, rows, heads / kvh) * kvh * split * PAIRS * (hd + 4) * sizeof(float);
+}
+
+int smc_launch_paged_prompt(smc_ctx *ctx, const smc_paged_view &c, const smc_paged_query &u, float *work, cudaStream_t s)
+{
+    const int group = u.heads / c.kvh, split = split_of(ctx, c.kvh, c.batch, c.rows, group, u.max_len);
+    const long long items = items_of(c.batch, c.rows, group);
+    if (items * c.kvh * split * (PAIRS / 8) > 0x7FFFFFFF || (long long)c.rows * group > 0x7FFFFFFF)
+        return smc_fail(ctx, SMC_E_UNSUPPORTED, "paged_attention: %d rows of %d sequences in one call", c.rows, c.batch);
+    auto go = [&](auto main, auto join, uint32_t smem) {
+        cudaFuncSetAttribute(main, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        smc_launch_dep(ctx->use_pdl, main, dim3((unsigned)(items * c.kvh * split)), dim3(THREADS), smem, s, c, u, (int)items, split, work, ctx->d_status);
+        if (split > 1) smc_launch_dep(ctx->use_pdl, join, dim3((unsigned)(items * c.kvh * (PAIRS / 8))), dim3(256), 0, s, c, u, (int)items, split, work);
+    };
+    if (u.bf16)
+        u.hd == 128 ? go(paged_prompt_kernel<bf16, 128>, paged_prompt_join_kernel<bf16, 128>, Shape<128, false>::SMEM)
+                    : go(paged_prompt_kernel<bf16, 64>, paged_prompt_join_kernel<bf16, 64>, Shape<64, false>::SMEM);
+    else
+        u.hd == 128 ? go(paged_prompt_kernel<float, 128>, paged_prompt_join_kernel<float, 128>, Shape<128, true>::SMEM)
+                    : go(paged_prompt_kernel<float, 64>, paged_prompt_join_kernel<float, 64>, Shape<64, true>::SMEM);
+    SMC_LAUNCH_CHECK(ctx);
+    return SMC_OK;
+}

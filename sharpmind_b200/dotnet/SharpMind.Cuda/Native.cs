@@ -160,7 +160,7 @@ internal static unsafe partial class Native
     [LibraryImport(Lib)] internal static partial int smc_paged_update_dev(nint ctx, in SmcPagedKv kv, in SmcPagedSeqs seqs, int dtype, nint dK, long kStride,
         nint dV, long vStride, nint dQ, long qStride, nint dQOut, int heads, nint dCos, nint dSin, int ropeDim, int tableRows, int neox, nint stream);
     [LibraryImport(Lib)] internal static partial int smc_paged_read_dev(nint ctx, in SmcPagedKv kv, nint dPages, int n, int dtype, nint dK, nint dV, nint stream);
-    [LibraryImport(Lib)] internal static partial long smc_paged_attention_work(nint ctx, in SmcPagedKv kv, int batch, int heads, int maxRows, int maxLen);
+    [LibraryImport(Lib)] internal static partial long smc_paged_attention_work(nint ctx, in SmcPagedKv kv, int batch, int rows, int heads, int maxRows, int maxLen);
     [LibraryImport(Lib)] internal static partial int smc_paged_attention_dev(nint ctx, in SmcPagedKv kv, in SmcPagedSeqs seqs, int dtype, nint dQ, long qStride,
         nint dOut, int heads, float scale, int window, int maxRows, int maxLen, nint dWork, long workBytes, nint stream);
 

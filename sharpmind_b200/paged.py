@@ -132,7 +132,7 @@ class PagedKVCache:
         most = 1 if row_start is None else rows if max_rows is None else max_rows
         long = seqs.width * self.page if max_len is None else max_len
         lib = self.ctx.lib
-        n = lib.smc_paged_attention_work(self.ctx.h, C.byref(self._kv), seqs.batch, heads, most, long)
+        n = lib.smc_paged_attention_work(self.ctx.h, C.byref(self._kv), seqs.batch, rows, heads, most, long)
         _require(n >= 0, f"max_rows {most} and max_len {long} do not describe a call")
         work = t.empty(n, dtype=t.uint8, device=self.device) if n else None
         rc = lib.smc_paged_attention_dev(self.ctx.h, C.byref(self._kv), C.byref(seqs), type_, q.data_ptr(), qs, out.data_ptr(), heads, scale, window, most, long,

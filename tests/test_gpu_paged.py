@@ -421,7 +421,7 @@ def test_the_library_refuses_what_it_has_no_kernel_for(cuda):
     x = torch.zeros((1, 4, 128), device="cuda")
 
     def attend(kv=p.cache._kv, seqs=s, dtype=0, q=x.data_ptr(), stride=512, out=x.data_ptr(), heads=4, window=0, most=1, long=20):
-        n = lib.smc_paged_attention_work(cuda.h, C.byref(kv), 1, heads, most, long)
+        n = lib.smc_paged_attention_work(cuda.h, C.byref(kv), 1, 1, heads, most, long)
         work = torch.empty(max(n, 16), dtype=torch.uint8, device="cuda")
         return lib.smc_paged_attention_dev(cuda.h, C.byref(kv), C.byref(seqs), dtype, q, stride, out, heads, 0.1, window, most, long, work.data_ptr(), max(n, 0), None)
 

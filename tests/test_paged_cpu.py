@@ -108,8 +108,8 @@ def test_the_library_refuses_without_a_context():
     from sharpmind_b200 import _lib
 
     lib, kv, sq = _lib.load(), paged._Kv(), paged._Seqs()
-    assert lib.smc_paged_attention_work(None, C.byref(kv), 1, 4, 1, 10) == -1
-    assert lib.smc_paged_attention_work(None, None, 1, 4, 1, 10) == -1
+    assert lib.smc_paged_attention_work(None, C.byref(kv), 1, 1, 4, 1, 10) == -1
+    assert lib.smc_paged_attention_work(None, None, 1, 1, 4, 1, 10) == -1
     assert lib.smc_paged_attention_dev(None, C.byref(kv), C.byref(sq), 0, None, 0, None, 4, 0.1, 0, 1, 10, None, 0, None) == 1
     assert lib.smc_paged_update_dev(None, C.byref(kv), C.byref(sq), 0, None, 0, None, 0, None, 0, None, 0, None, None, 0, 0, 0, None) == 1
     assert lib.smc_paged_read_dev(None, C.byref(kv), None, 1, 0, None, None, None) == 1
