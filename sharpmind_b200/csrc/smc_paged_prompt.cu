@@ -61,6 +61,23 @@ __device__ __forceinline__ uint32_t rest_bits(float a, float b, uint32_t hi)
     const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
     return half2_bits(a - h.x, b - h.y);
 }
+// two fp32 operations an instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
 __host__ __device__ constexpr uint32_t idesc_f16(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TILE >> 4) << 24); }
 
 // What a CTA does: pairs [m0, m0 + pairs) of sequence s and head h; key tiles [kv0, kv0 + n[t]) of tile t, of which this piece takes [i0, i1).
@@ -206,20 +223,33 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
             const float4 *sc = reinterpret_cast<const float4 *>(smem + S::OFF_SC) + (it % SC_SLOTS) * G;
             smc_tc_wait_ld();
             const bool inner = key0 + KT <= lowest + 1 && (u.window <= 0 || key0 > highest - u.window);
+            const int hi = inner ? KT : pos - key0, lo = !inner && u.window > 0 ? hi - u.window : -1;  // keys lo + 1 .. hi of the tile are seen
             if (!inner) {
-                const int hi = pos - key0, lo = u.window > 0 ? hi - u.window : -1;
 #pragma unroll
                 for (int k = 0; k < KT; ++k)
-                    if (k > hi || k <= lo) s[k] = 0xFF800000u;  // -infinity
+                    if (k > hi) s[k] = 0xFF800000u;  // -infinity
+                if (lo >= 0) {
+#pragma unroll
+                    for (int k = 0; k < KT; ++k)
+                        if (k <= lo) s[k] = 0xFF800000u;
+                }
             }
+            // scales of 16 keys, for this row: a factor above 0, so that hidden keys stay -infinity; nothing of keys that are all hidden
+            auto scales = [&](int k) {
+                float4 x = sc[k];
+                x.x = fmaxf(x.x * rowf, 1e-37f);
+                if (16 * k > hi || 16 * k + 15 <= lo) x.y = -INFINITY, x.z = 0.0f;
+                return x;
+            };
             float top = -INFINITY;
 #pragma unroll
             for (int k = 0; k < G; ++k) {
-                const float4 x = sc[k];
-                float gm = __uint_as_float(s[16 * k]);
+                float m4[4];
 #pragma unroll
-                for (int e = 1; e < 16; ++e) gm = fmaxf(gm, __uint_as_float(s[16 * k + e]));
-                top = fmaxf(top, fmaf(gm, x.x * rowf, x.y));  // (hidden keys, -inf, times 0 or an undefined scale: not a number, which a maximum drops)
+                for (int e = 0; e < 4; ++e)
+                    m4[e] = fmaxf(fmaxf(__uint_as_float(s[16 * k + e]), __uint_as_float(s[16 * k + 4 + e])), fmaxf(__uint_as_float(s[16 * k + 8 + e]), __uint_as_float(s[16 * k + 12 + e])));
+                const float4 x = scales(k);
+                top = fmaxf(top, fmaf(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), x.x, x.y));  // (what is not a number a maximum drops)
             }
             float corr = 1.0f;
             if (top > R + R_ABOVE) {
@@ -245,26 +275,21 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
             uint32_t rest[SPLIT ? KT / 2 : 1];
 #pragma unroll
             for (int k = 0; k < G; ++k) {
-                const float4 x = sc[k];
-                const float f = x.x * rowf, b = x.y - ref;
-                float w[16], sum = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) w[e] = ex2(fmaf(__uint_as_float(s[16 * k + e]), f, b));
-                if (!inner) {
-                    const int hi = pos - key0 - 16 * k, lo = u.window > 0 ? hi - u.window : -1;
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (e > hi || e <= lo) w[e] = 0.0f;
-                }
-#pragma unroll
-                for (int e = 0; e < 16; ++e) sum += w[e];
-                // (a row that sees none of these keys takes nothing of their scale, which may be undefined)
-                l = inner ? fmaf(sum, x.z, l) : l + (sum == 0.0f ? 0.0f : sum * x.z);
+                const float4 x = scales(k);
+                const float2 f = make_float2(x.x, x.x), bias = make_float2(x.y - ref, x.y - ref);
+                float2 w[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const uint32_t hi = half2_bits(w[2 * e], w[2 * e + 1]);
-                    if constexpr (SPLIT) rest[8 * k + e] = rest_bits(w[2 * e], w[2 * e + 1], hi);
-                    s[8 * k + e] = hi;  // (the scores there are used up)
+                    w[e] = fma2(make_float2(__uint_as_float(s[16 * k + 2 * e]), __uint_as_float(s[16 * k + 2 * e + 1])), f, bias);
+                    w[e].x = ex2(w[e].x), w[e].y = ex2(w[e].y);
+                }
+                const float2 sum = add2(add2(add2(w[0], w[1]), add2(w[2], w[3])), add2(add2(w[4], w[5]), add2(w[6], w[7])));
+                l = fmaf(sum.x + sum.y, x.z, l);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t hi16 = half2_bits(w[e].x, w[e].y);
+                    if constexpr (SPLIT) rest[8 * k + e] = rest_bits(w[e].x, w[e].y, hi16);
+                    s[8 * k + e] = hi16;  // (the scores there are used up)
                 }
             }
 #pragma unroll
@@ -307,10 +332,18 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
     } else if (warp < MMA_WARP) {
         // ---------------------------------------------------------------- codes to fp16
         asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-        const int w = warp - CONV_WARP, page = 1 << c.shift;
-        constexpr int UNITS = KT * HD / 16 / 128;  // 16 codes a thread each
+        const int w = warp - CONV_WARP, page = 1 << c.shift, r8 = lane & 7, q4 = lane >> 3;
+        constexpr int UNITS = KT * HD / 16 / 128;  // of 16 codes a thread: 8 keys x 64 dims, 8 dims x 64 keys a warp
+        constexpr int IN_K = HD / 64, IN_V = KT / 64, STEP_K = 4 / IN_K, STEP_V = 4 / IN_V;
+        // unit x of this warp: keys 8 (w / IN_K + STEP_K x) .., dims 64 (w % IN_K) + 16 q4 ..; dims 8 (w / IN_V + STEP_V x) .., keys 64 (w % IN_V) + 16 q4 ..
         const int hi = min(j.len, j.len - j.n_rows + (j.m0 + j.pairs - 1) / group + 1);  // keys [from, hi) count
-        // page of this lane's group of 16 keys (lane % G) of tile i, or -1
+        const uint32_t stride = (uint32_t)(c.kvh * HD) << c.shift;                         // bytes of a page
+        const uint8_t *k_base = c.k + ((size_t)j.h * HD << c.shift) + 64 * (w % IN_K) + 16 * q4, *v_base = c.v + ((size_t)j.h * HD << c.shift) + ((size_t)(8 * (w / IN_V) + r8) << c.shift);
+        const int v_group = 4 * (w % IN_V) + q4;
+        const uint32_t swizzle = (uint32_t)(r8 * 128 + ((2 * q4) ^ r8) * 16), flip = (uint32_t)((2 * q4 ^ r8) * 16) ^ (uint32_t)(((2 * q4 + 1) ^ r8) * 16);
+        const uint32_t k_dst = sbase + S::OFF_K + (uint32_t)((w % IN_K) * KT * 128 + w / IN_K * 1024), v_dst = sbase + S::OFF_V + (uint32_t)((w % IN_V) * HD * 128 + w / IN_V * 1024);
+        // Page of this lane's group of 16 keys (lane % G) of tile i, or -1.  Codes of page 0 stand in for those of a page that is not there: nothing of a
+        // key that no row sees reaches a result, and undefined codes among the values are made zeros below.
         auto page_of = [&](int i) {
             const int key = (j.kv0 + i) * KT + 16 * (lane % G), p0 = key >> c.shift << c.shift;
             if (i >= j.i1 || p0 + page <= j.from || p0 >= hi) return -1;  // (pages that left the window may have gone to another sequence)
@@ -318,78 +351,66 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
             if (id < 0) *status = SMC_STATUS_PAGED;
             return id;
         };
-        const int r8 = lane & 7, q4 = lane >> 3;
-        auto fetch = [&](const uint8_t *base, int ids, bool values, int i, int x) {
-            const int inner = values ? KT / 64 : HD / 64, big = x / inner, half = x - big * inner;
-            const int group16 = values ? 4 * half + q4 : big >> 1;  // of the tile's keys
-            const int id = __shfl_sync(0xFFFFFFFFu, ids, group16);
-            uint4 v = make_uint4(0, 0, 0, 0);
-            const int key = (j.kv0 + i) * KT + (values ? 16 * group16 : 8 * big + r8);
-            if (id >= 0) {
-                const uint8_t *p = base + ((size_t)id * c.kvh + j.h) * ((size_t)HD << c.shift);
-                p += values ? ((8 * big + r8) << c.shift) + (key & (page - 1)) : (key & (page - 1)) * HD + 64 * half + 16 * q4;
-                v = __ldcg(reinterpret_cast<const uint4 *>(p));
-                if (values) {  // values that do not count are zeros whatever their bytes are: the weights there are 0, and codes may be undefined
-                    if (key < j.from || key + 16 > hi) {
-                        uint32_t *b = &v.x;
-#pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            if (key + e < j.from || key + e >= hi) b[e >> 2] &= ~(0xFFu << (8 * (e & 3)));
-                    }
-                } else if (key >= hi) {
-                    v = make_uint4(0, 0, 0, 0);
-                }
-            }
-            return v;
+        auto scales_of = [&](int id) { return id < 0 ? make_float2(0.0f, 0.0f) : *reinterpret_cast<const float2 *>(c.scales + 2 * ((size_t)id * c.kvh + j.h)); };
+        auto fetch_k = [&](int ids, int x) {
+            const int in_tile = 8 * (w / IN_K + STEP_K * x), id = max(__shfl_sync(0xFFFFFFFFu, ids, in_tile >> 4), 0);
+            return __ldcg(reinterpret_cast<const uint4 *>(k_base + (size_t)(uint32_t)id * stride + ((in_tile & (page - 1)) + r8) * HD));
         };
-        auto place = [&](uint32_t stage, bool values, int x, const uint4 &v) {
-            const int inner = values ? KT / 64 : HD / 64, big = x / inner, half = x - big * inner;
-            const uint32_t row = stage + (uint32_t)half * (uint32_t)((values ? HD : KT) * 128) + (uint32_t)big * 1024u + (uint32_t)r8 * 128u;
+        auto fetch_v = [&](const uint8_t *v_page, int x) { return __ldcg(reinterpret_cast<const uint4 *>(v_page + ((8 * STEP_V * x) << c.shift))); };
+        auto place = [&](uint32_t at, const uint4 &v) {
             const uint32_t raw[4] = {v.x, v.y, v.z, v.w};
             uint32_t h[8];
 #pragma unroll
             for (int e = 0; e < 4; ++e) h[2 * e] = smc_e4m3x2_half2(raw[e] & 0xFFFFu), h[2 * e + 1] = smc_e4m3x2_half2(raw[e] >> 16);
-            sts128(row + (uint32_t)(((2 * q4) ^ r8) << 4), h[0], h[1], h[2], h[3]);
-            sts128(row + (uint32_t)(((2 * q4 + 1) ^ r8) << 4), h[4], h[5], h[6], h[7]);
-        };
-        auto scales = [&](int i, int ids) {
-            if (w == 0 && lane < G) {
-                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (ids >= 0) {
-                    const float2 s2 = *reinterpret_cast<const float2 *>(c.scales + 2 * ((size_t)ids * c.kvh + j.h));
-                    // (a power of two's exponent; an undefined scale stays what it is)
-                    x = make_float4(s2.x, s2.y == s2.y ? (float)((int)(__float_as_uint(s2.y) >> 23) - 127) : s2.y, 1.0f / s2.y, 0.0f);
-                }
-                reinterpret_cast<float4 *>(smem + S::OFF_SC)[((i - j.i0) % SC_SLOTS) * G + lane] = x;
-            }
+            sts128(at, h[0], h[1], h[2], h[3]);
+            sts128(at ^ flip, h[4], h[5], h[6], h[7]);
         };
         uint4 raw[UNITS];
-        int ids = page_of(j.i0), ids_next = page_of(j.i0 + 1);
+        int now = page_of(j.i0), next = page_of(j.i0 + 1);
+        float2 sc = scales_of(now);
 #pragma unroll
-        for (int x = 0; x < UNITS; ++x) raw[x] = fetch(c.k, ids, false, j.i0, w + 4 * x);
+        for (int x = 0; x < UNITS; ++x) raw[x] = fetch_k(now, x);
 #pragma unroll 1
         for (int i = j.i0; i < j.i1; ++i) {
-            const int it = i - j.i0, st = it & 1;
+            const int it = i - j.i0, st = it & 1, key0 = (j.kv0 + i) * KT;
             const uint32_t parity = (uint32_t)(it >> 1) ^ 1u;  // (a fresh barrier passes the first)
+            const int v_id = __shfl_sync(0xFFFFFFFFu, now, v_group);
+            const uint8_t *v_page = v_base + (size_t)(uint32_t)max(v_id, 0) * stride + ((16 * v_group) & (page - 1));
             wait(K_EMPTY + st, parity);
-            scales(i, ids);
+            if (w == 0 && lane < G) {
+                // scale of keys; log2 and reciprocal of that of values (a power of two's exponent).  An undefined one of either makes the second undefined
+                const float both = sc.x + sc.y, e = (float)((int)(__float_as_uint(sc.y) >> 23) - 127);
+                reinterpret_cast<float4 *>(smem + S::OFF_SC)[(it % SC_SLOTS) * G + lane] =
+                    now < 0 ? make_float4(0.0f, -INFINITY, 0.0f, 0.0f) : make_float4(sc.x, both == both ? e : both, 1.0f / sc.y, 0.0f);
+            }
 #pragma unroll
             for (int x = 0; x < UNITS; ++x) {  // as a unit's registers are free, they take the codes of the next half
-                place(sbase + S::OFF_K + (uint32_t)st * S::STAGE, false, w + 4 * x, raw[x]);
-                raw[x] = fetch(c.v, ids, true, i, w + 4 * x);
+                place(k_dst + (uint32_t)st * S::STAGE + (uint32_t)(STEP_K * x) * 1024u + swizzle, raw[x]);
+                raw[x] = fetch_v(v_page, x);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             arrive(K_FULL + st);
             const int after = page_of(i + 2);
+            sc = scales_of(next);
             wait(V_EMPTY + st, parity);
+            if (key0 < j.from || key0 + KT > hi || __any_sync(0xFFFFFFFFu, now < 0)) {  // values of keys that do not count are zeros
+                uint32_t keep[4] = {};
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int key = key0 + 16 * v_group + e;
+                    if (v_id >= 0 && key >= j.from && key < hi) keep[e >> 2] |= 0xFFu << (8 * (e & 3));
+                }
+#pragma unroll
+                for (int x = 0; x < UNITS; ++x) raw[x].x &= keep[0], raw[x].y &= keep[1], raw[x].z &= keep[2], raw[x].w &= keep[3];
+            }
 #pragma unroll
             for (int x = 0; x < UNITS; ++x) {
-                place(sbase + S::OFF_V + (uint32_t)st * S::STAGE, true, w + 4 * x, raw[x]);
-                raw[x] = fetch(c.k, ids_next, false, i + 1, w + 4 * x);
+                place(v_dst + (uint32_t)st * S::STAGE + (uint32_t)(STEP_V * x) * 1024u + swizzle, raw[x]);
+                raw[x] = fetch_k(next, x);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             arrive(V_FULL + st);
-            ids = ids_next, ids_next = after;
+            now = next, next = after;
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
