@@ -1,43 +1,70 @@
 // Attention of many rows over the paged cache (a prompt, a chunk of one, long drafts) on the fifth-generation tensor cores.
 //
-// One CTA = up to 256 (row, query head) pairs of one sequence and KV head, two tiles of 128, a thread a pair; keys in tiles of KT.  The codes are brought as
+// One CTA = up to 256 (row, query head) pairs of one sequence and KV head, two tiles of 128, a thread a pair; keys in steps of 64.  The codes are brought as
 // they lie in their pages, turned to fp16 (exact) by four warps and stored as 128-byte-swizzled K-major tiles, once for all heads of a group and both
 // tiles.  Scores S = Q K^T and outputs O += P V are tcgen05.mma, fp16 with fp32 sums in tensor memory, P in the columns that S leaves:
-//   bfloat16  queries exact in fp16 after a power of two per row, weights rounded to 11 bits; KT = 128
-//   fp32      queries and weights as hi + lo, 22 bits, two products each; KT = 64
+//   bfloat16  queries exact in fp16 after a power of two per row, weights rounded to 11 bits
+//   fp32      queries and weights as hi + lo, 22 bits, two products each
 // With the pages' scales, constant over 16 keys:  y = S f + b, f = s_k * row factor, b = log2(s_v);  w = 2^(y - R);  l = sum w / s_v;  out = O / l.
 // R follows the running maximum of y only where that gets more than 2^15 above it (then to 2^8 below), so O, in tensor memory, is rarely
 // multiplied again; a weight stays under 2^15 and counts down to 2^-24.
-// Warp roles:  0 .. 3, 4 .. 7  softmax of tile 0, 1      8 .. 11  codes to fp16      12  MMA issue
-// MMA order per key tile i:  O0 += P0(i) V(i), S0(i + 1), O1 += P1(i) V(i), S1(i + 1): one tile's products run under the other's softmax.  MMAs of one
-// thread run in order, so S(i + 1) may overwrite P(i), and a softmax that has S(i + 1) may touch O.
-// Few pairs: the key tiles are split over CTAs, whose partial results a second kernel joins.
+// Warp roles:  0 .. 3, 4 .. 7  softmax of tile 0, 1      8 .. 11  codes to fp16      12, 13  MMA issue of tile 0, 1
+// Scores have two buffers a tile, so a softmax finds its next ones there.
+// Few pairs: the steps are split over CTAs, whose partial results a second kernel joins.
 #include "smc_paged.cuh"
 #include "smc_tc.cuh"
 
 namespace {
 
-constexpr int PAIRS = 256, TILE = 128, SOFT_WARPS = 8, CONV_WARP = 8, MMA_WARP = 12, THREADS = 512, SC_SLOTS = 4;
+constexpr int PAIRS = 256, TILE = 128, KT = 64, G = KT / 16, SOFT_WARPS = 8, CONV_WARP = 8, MMA_WARP = 12, THREADS = 32 * (MMA_WARP + 2), SC_SLOTS = 8;
 constexpr float R_ABOVE = 15.0f, R_BELOW = 8.0f;
+
+// A wait names a phase by its parity: no barrier passes a phase before its waiter has seen the one before.  (PV_DONE may for a softmax, which looks
+// at it only in step i for the product of step i - 1, where neither the one before can be missing nor the one after be there.)
+enum { K_FULL = 0, K_EMPTY = 4, V_FULL = 8, V_EMPTY = 12, S_FULL = 16, P_FULL = 20 /* [tile][step parity] */, PV_DONE = 24, Q_FULL = 26, O_FULL = 28, BARS = 30 };
 
 template <int HD, bool SPLIT>
 struct Shape {
-    static constexpr int PLANES = SPLIT ? 2 : 1, KT = SPLIT ? 64 : 128;
+    static constexpr int PLANES = SPLIT ? 2 : 1, NK = 4, NV = SPLIT ? 2 : 4;
     static constexpr uint32_t SUB_Q = TILE * 128, Q_PLANE = HD / 64 * SUB_Q, Q_TILE = PLANES * Q_PLANE;
-    static constexpr uint32_t STAGE = KT * HD * 2;  // fp16 keys or values of a tile
-    static constexpr uint32_t OFF_K = 2 * Q_TILE, OFF_V = OFF_K + 2 * STAGE, OFF_SC = OFF_V + 2 * STAGE, OFF_BAR = OFF_SC + SC_SLOTS * (KT / 16) * 16, SMEM = OFF_BAR + 256;
-    static constexpr uint32_t COL_S = 0, COL_O = 256, COLS = 512;
-    static_assert(SMEM <= 227 * 1024 && COL_O + 2 * HD <= COLS && 2 * KT <= COL_O, "");
+    static constexpr uint32_t STAGE = KT * HD * 2;  // fp16 keys or values of a step
+    static constexpr uint32_t OFF_K = 2 * Q_TILE, OFF_V = OFF_K + NK * STAGE, OFF_SC = OFF_V + NV * STAGE, OFF_BAR = OFF_SC + SC_SLOTS * G * 16, SMEM = OFF_BAR + 256;
+    static constexpr uint32_t COL_S = 0, COL_O = 4 * KT, COLS = 512;  // scores [tile][step parity]
+    static_assert(BARS * 8 + 8 <= 256 && SMEM <= 227 * 1024 && COL_O + 2 * HD <= COLS && NK < SC_SLOTS, "");
 };
-enum { K_FULL = 0, K_EMPTY = 2, V_FULL = 4, V_EMPTY = 6, S_FULL = 8, P_FULL = 10, O_FULL = 12, Q_FULL = 14, BARS = 16 };
-
-__device__ __forceinline__ void mma_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)  // A in tensor memory
+// tcgen05.mma whose operands are known at compile time, up to the shared memory's base: operands that come through registers take an issuing
+// thread some 140 clocks an MMA (measured here), these less than the MMA itself.  D, A_COL: columns of tensor memory, all of which is the CTA's, so it starts
+// at 0; A, B: byte offsets of swizzled tiles; base: low word of the descriptor of offset 0.
+constexpr uint32_t DESC_HIGH = (1024u >> 4) | (1u << 14) | (2u << 29);
+template <uint32_t D, uint32_t A, uint32_t B, uint32_t IDESC>
+__device__ __forceinline__ void mma_ss(uint32_t base, uint32_t accumulate)
 {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p;\n\t.reg .b32 a, b, d, i;\n\t.reg .b64 x, y;\n\tadd.u32 a, %0, %2;\n\tadd.u32 b, %0, %3;\n\tmov.b64 x, {a, %6};\n\tmov.b64 y, {b, %6};\n\t"
+        "mov.u32 d, %4;\n\tmov.u32 i, %5;\n\tsetp.ne.b32 p, %1, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [d], x, y, i, p;\n\t}" ::"r"(base),
+        "r"(accumulate), "n"(A >> 4), "n"(B >> 4), "n"(D), "n"(IDESC), "n"(DESC_HIGH)
         : "memory");
+}
+template <uint32_t D, uint32_t A_COL, uint32_t B, uint32_t IDESC>
+__device__ __forceinline__ void mma_ts(uint32_t base, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b32 a, b, d, i;\n\t.reg .b64 y;\n\tadd.u32 b, %0, %3;\n\tmov.b64 y, {b, %6};\n\tmov.u32 a, %2;\n\t"
+        "mov.u32 d, %4;\n\tmov.u32 i, %5;\n\tsetp.ne.b32 p, %1, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [d], [a], y, i, p;\n\t}" ::"r"(base),
+        "r"(accumulate), "n"(A_COL), "n"(B >> 4), "n"(D), "n"(IDESC), "n"(DESC_HIGH)
+        : "memory");
+}
+// f(integral constants 0 .. N - 1)
+template <int I> struct ic {
+    static constexpr int v = I;
+};
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void each(F &&f)
+{
+    if constexpr (I < N) {
+        f(ic<I>());
+        each<N, I + 1>(f);
+    }
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r)
 {
@@ -80,11 +107,71 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b)
 }
 __host__ __device__ constexpr uint32_t idesc_f16(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TILE >> 4) << 24); }
 
+// One thread issues a tile's MMAs: scores of two steps ahead; then, step by step, O += P(i) V(i) and the scores of step i + 2, which take the buffer that P(i) was
+// in.  The wait for that product delays nobody: the softmax has step i + 1 meanwhile, and the tensor cores the other tile's MMAs.
+template <int HD, bool SPLIT, int TILE_NO>
+__device__ __forceinline__ void issue_mmas(uint32_t sbase, int mine, int n, uint32_t bars, volatile uint32_t *abort_flag, int *status)
+{
+    using S = Shape<HD, SPLIT>;
+    constexpr int UNROLL = S::NK;  // stages are constants
+    static_assert(S::NK % 2 == 0 && S::NK % S::NV == 0, "");
+    const uint32_t base = ((sbase >> 4) & 0x3FFFu) | (1u << 16);
+    auto wait = [&](int i, uint32_t parity) { smc_tc_wait(bars + 8u * (uint32_t)i, parity & 1u, abort_flag, status); };
+    auto scores = [&](auto stage, int it) {  // it % NK = stage
+        constexpr int st = decltype(stage)::v;
+        wait(K_FULL + st, (uint32_t)(it / S::NK));
+        if (it >= mine) {  // the other tile goes on
+            smc_mbar_arrive(bars + 8u * (K_EMPTY + st));
+            return;
+        }
+        smc_tc_fence_after();
+        each<S::PLANES * (HD / 16)>([&](auto x) {
+            constexpr int p = S::PLANES - 1 - decltype(x)::v / (HD / 16), ks = decltype(x)::v % (HD / 16);  // smallest products first
+            mma_ss<S::COL_S + (2 * TILE_NO + st % 2) * KT, TILE_NO * S::Q_TILE + p * S::Q_PLANE + ks / 4 * S::SUB_Q + ks % 4 * 32,
+                   S::OFF_K + st * S::STAGE + ks / 4 * (KT * 128) + ks % 4 * 32, idesc_f16(KT)>(base, decltype(x)::v > 0);
+        });
+        smc_tc_commit(bars + 8u * (S_FULL + 2 * TILE_NO + st % 2));
+        smc_tc_commit(bars + 8u * (K_EMPTY + st));
+    };
+    auto outputs = [&](auto stage, int it) {
+        constexpr int st = decltype(stage)::v, vs = st % S::NV;
+        wait(V_FULL + vs, (uint32_t)(it / S::NV));
+        if (it >= mine) {
+            smc_mbar_arrive(bars + 8u * (V_EMPTY + vs));
+            return;
+        }
+        wait(P_FULL + 2 * TILE_NO + st % 2, (uint32_t)(it >> 1));
+        smc_tc_fence_after();
+        each<S::PLANES * (KT / 16)>([&](auto x) {
+            constexpr int p = S::PLANES - 1 - decltype(x)::v / (KT / 16), kk = decltype(x)::v % (KT / 16);
+            mma_ts<S::COL_O + TILE_NO * HD, S::COL_S + (2 * TILE_NO + st % 2) * KT + p * (KT / 2) + kk * 8, S::OFF_V + vs * S::STAGE + kk * 32, idesc_f16(HD)>(
+                base, decltype(x)::v > 0 || it > 0);
+        });
+        smc_tc_commit(bars + 8u * (PV_DONE + TILE_NO));
+        if (it + 1 == mine) smc_tc_commit(bars + 8u * (O_FULL + TILE_NO));
+        smc_tc_commit(bars + 8u * (V_EMPTY + vs));
+    };
+    if (mine > 0) wait(Q_FULL + TILE_NO, 0u);
+    scores(ic<0>(), 0);
+    if (n > 1) scores(ic<1>(), 1);
+#pragma unroll 1
+    for (int it = 0; it < n; it += UNROLL)
+        each<UNROLL>([&](auto x) {
+            constexpr int st = decltype(x)::v;
+            const int i = it + st;
+            if (i >= n) return;
+            outputs(x, i);
+            if (i + 2 < n) {
+                if (i + 2 < mine) wait(PV_DONE + TILE_NO, (uint32_t)i);
+                scores(ic<(st + 2) % UNROLL>(), i + 2);
+            }
+        });
+}
+
 // What a CTA does: pairs [m0, m0 + pairs) of sequence s and head h; key tiles [kv0, kv0 + n[t]) of tile t, of which this piece takes [i0, i1).
 struct Job {
     int s, h, m0, pairs, len, n_rows, r0, from, kv0, n0, n1, i0, i1, piece, pieces;
 };
-template <int KT>
 __device__ __forceinline__ bool job_of(const smc_paged_view &c, const smc_paged_query &u, int item, int h, int piece, int split, Job &j, int *status)
 {
     const int group = u.heads / c.kvh;
@@ -118,7 +205,6 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
 {
     constexpr bool SPLIT = sizeof(T) == 4;
     using S = Shape<HD, SPLIT>;
-    constexpr int KT = S::KT, G = KT / 16;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sbase = smc_smem_u32(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -140,16 +226,17 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
         const int piece = b % split;
         b /= split;
         const int h = b % c.kvh, item = items - 1 - b / c.kvh;  // later rows see more keys: they start first
-        if (!job_of<KT>(c, u, item, h, piece, split, j, threadIdx.x == 0 ? status : nullptr)) {  // (the same for all threads)
+        if (!job_of(c, u, item, h, piece, split, j, threadIdx.x == 0 ? status : nullptr)) {  // (the same for all threads)
             asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
             return;
         }
     }
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2; ++i) {
-            smc_mbar_init(bar(K_FULL + i), 4), smc_mbar_init(bar(K_EMPTY + i), 1), smc_mbar_init(bar(V_FULL + i), 4), smc_mbar_init(bar(V_EMPTY + i), 1);
-            smc_mbar_init(bar(S_FULL + i), 1), smc_mbar_init(bar(P_FULL + i), 4), smc_mbar_init(bar(O_FULL + i), 1), smc_mbar_init(bar(Q_FULL + i), 4);
-        }
+        const uint32_t readers = j.pairs > TILE ? 2u : 1u;
+        for (int i = 0; i < S::NK; ++i) smc_mbar_init(bar(K_FULL + i), 4), smc_mbar_init(bar(K_EMPTY + i), readers);
+        for (int i = 0; i < S::NV; ++i) smc_mbar_init(bar(V_FULL + i), 4), smc_mbar_init(bar(V_EMPTY + i), readers);
+        for (int i = 0; i < 4; ++i) smc_mbar_init(bar(S_FULL + i), 1), smc_mbar_init(bar(P_FULL + i), 4);
+        for (int i = 0; i < 2; ++i) smc_mbar_init(bar(PV_DONE + i), 1), smc_mbar_init(bar(O_FULL + i), 1), smc_mbar_init(bar(Q_FULL + i), 4);
         *abort_flag = 0;
         smc_fence_barrier_init();
     }
@@ -167,11 +254,10 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
     const int stop0 = min(j.n0, j.i1), stop1 = two ? j.i1 : j.i0;  // tile t takes [i0, stop)
 
     if (warp < SOFT_WARPS) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
         const int t = warp >> 2, rl = 32 * (warp & 3) + lane, m = t * TILE + rl, stop = t ? stop1 : stop0;
         const bool real = m < j.pairs;
         const int pair = j.m0 + (real ? m : 0), tok = pair / group, head = j.h * group + pair - tok * group;
-        const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16), col_s = lanes + S::COL_S + (uint32_t)(t * KT), col_o = lanes + S::COL_O + (uint32_t)(t * HD);
+        const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16), col_s0 = lanes + S::COL_S + (uint32_t)(2 * t * KT), col_o = lanes + S::COL_O + (uint32_t)(t * HD);
         const int pos = j.len - j.n_rows + tok;
         float rowf = 0.0f, R = -INFINITY, l = 0.0f;
         if (stop > j.i0) {
@@ -215,7 +301,8 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
 #pragma unroll 1
         for (int i = j.i0; i < stop; ++i) {
             const int it = i - j.i0, key0 = (j.kv0 + i) * KT;
-            wait(S_FULL + t, (uint32_t)it);
+            const uint32_t col_s = col_s0 + (uint32_t)((it & 1) * KT);
+            wait(S_FULL + 2 * t + (it & 1), (uint32_t)(it >> 1));
             smc_tc_fence_after();
             uint32_t s[KT];
 #pragma unroll
@@ -241,16 +328,18 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
                 if (16 * k > hi || 16 * k + 15 <= lo) x.y = -INFINITY, x.z = 0.0f;
                 return x;
             };
-            float top = -INFINITY;
+            float4 x[G];
+            float y[G];
 #pragma unroll
             for (int k = 0; k < G; ++k) {
+                x[k] = scales(k);
                 float m4[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     m4[e] = fmaxf(fmaxf(__uint_as_float(s[16 * k + e]), __uint_as_float(s[16 * k + 4 + e])), fmaxf(__uint_as_float(s[16 * k + 8 + e]), __uint_as_float(s[16 * k + 12 + e])));
-                const float4 x = scales(k);
-                top = fmaxf(top, fmaf(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), x.x, x.y));  // (what is not a number a maximum drops)
+                y[k] = fmaf(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), x[k].x, x[k].y);
             }
+            const float top = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));  // (what is not a number a maximum drops)
             float corr = 1.0f;
             if (top > R + R_ABOVE) {
                 const float was = R;
@@ -260,6 +349,8 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
             if (__any_sync(0xFFFFFFFFu, corr != 1.0f)) {
                 l *= corr;
                 if (it > 0) {
+                    wait(PV_DONE + t, (uint32_t)(it - 1));  // (the one before that: these scores waited for it)
+                    smc_tc_fence_after();
 #pragma unroll 1
                     for (int k = 0; k < HD; k += 16) {
                         uint32_t o[16];
@@ -275,8 +366,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
             uint32_t rest[SPLIT ? KT / 2 : 1];
 #pragma unroll
             for (int k = 0; k < G; ++k) {
-                const float4 x = scales(k);
-                const float2 f = make_float2(x.x, x.x), bias = make_float2(x.y - ref, x.y - ref);
+                const float2 f = make_float2(x[k].x, x[k].x), bias = make_float2(x[k].y - ref, x[k].y - ref);
                 float2 w[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
@@ -284,7 +374,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
                     w[e].x = ex2(w[e].x), w[e].y = ex2(w[e].y);
                 }
                 const float2 sum = add2(add2(add2(w[0], w[1]), add2(w[2], w[3])), add2(add2(w[4], w[5]), add2(w[6], w[7])));
-                l = fmaf(sum.x + sum.y, x.z, l);
+                l = fmaf(sum.x + sum.y, x[k].z, l);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const uint32_t hi16 = half2_bits(w[e].x, w[e].y);
@@ -299,10 +389,10 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
             }
             tmem_wait_st();
             smc_tc_fence_before();
-            arrive(P_FULL + t);
+            arrive(P_FULL + 2 * t + (it & 1));
         }
         if (stop > j.i0) {
-            wait(O_FULL + t, 0);
+            wait(O_FULL + t, 0u);
             smc_tc_fence_after();
             const float norm = j.pieces > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
             T *dst = static_cast<T *>(u.out) + ((size_t)(j.r0 + tok) * u.heads + head) * HD;
@@ -331,7 +421,6 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
         }
     } else if (warp < MMA_WARP) {
         // ---------------------------------------------------------------- codes to fp16
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         const int w = warp - CONV_WARP, page = 1 << c.shift, r8 = lane & 7, q4 = lane >> 3;
         constexpr int UNITS = KT * HD / 16 / 128;  // of 16 codes a thread: 8 keys x 64 dims, 8 dims x 64 keys a warp
         constexpr int IN_K = HD / 64, IN_V = KT / 64, STEP_K = 4 / IN_K, STEP_V = 4 / IN_V;
@@ -365,35 +454,40 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
             sts128(at, h[0], h[1], h[2], h[3]);
             sts128(at ^ flip, h[4], h[5], h[6], h[7]);
         };
-        uint4 raw[UNITS];
-        int now = page_of(j.i0), next = page_of(j.i0 + 1);
-        float2 sc = scales_of(now);
+        // keys two steps ahead of the values, as the MMAs want them; codes of the next step of each are on their way meanwhile
+        uint4 raw_k[UNITS], raw_v[UNITS];
+        int id_v, id_next, id_k = page_of(j.i0);  // pages of the next values, of those after, and of the next keys
+        float2 sc = scales_of(id_k);
+        auto next_k = [&](int ids) {
 #pragma unroll
-        for (int x = 0; x < UNITS; ++x) raw[x] = fetch_k(now, x);
-#pragma unroll 1
-        for (int i = j.i0; i < j.i1; ++i) {
-            const int it = i - j.i0, st = it & 1, key0 = (j.kv0 + i) * KT;
-            const uint32_t parity = (uint32_t)(it >> 1) ^ 1u;  // (a fresh barrier passes the first)
-            const int v_id = __shfl_sync(0xFFFFFFFFu, now, v_group);
-            const uint8_t *v_page = v_base + (size_t)(uint32_t)max(v_id, 0) * stride + ((16 * v_group) & (page - 1));
-            wait(K_EMPTY + st, parity);
+            for (int x = 0; x < UNITS; ++x) raw_k[x] = fetch_k(ids, x);
+        };
+        auto next_v = [&](int ids) {
+            const uint8_t *v_page = v_base + (size_t)(uint32_t)max(__shfl_sync(0xFFFFFFFFu, ids, v_group), 0) * stride + ((16 * v_group) & (page - 1));
+#pragma unroll
+            for (int x = 0; x < UNITS; ++x) raw_v[x] = fetch_v(v_page, x);
+        };
+        int k_stage = 0, v_stage = 0;
+        uint32_t k_phase = 1, v_phase = 1;  // (a fresh barrier passes the first)
+        auto put_k = [&](int it, int ids) {
+            wait(K_EMPTY + k_stage, k_phase);
             if (w == 0 && lane < G) {
                 // scale of keys; log2 and reciprocal of that of values (a power of two's exponent).  An undefined one of either makes the second undefined
                 const float both = sc.x + sc.y, e = (float)((int)(__float_as_uint(sc.y) >> 23) - 127);
                 reinterpret_cast<float4 *>(smem + S::OFF_SC)[(it % SC_SLOTS) * G + lane] =
-                    now < 0 ? make_float4(0.0f, -INFINITY, 0.0f, 0.0f) : make_float4(sc.x, both == both ? e : both, 1.0f / sc.y, 0.0f);
+                    ids < 0 ? make_float4(0.0f, -INFINITY, 0.0f, 0.0f) : make_float4(sc.x, both == both ? e : both, 1.0f / sc.y, 0.0f);
             }
 #pragma unroll
-            for (int x = 0; x < UNITS; ++x) {  // as a unit's registers are free, they take the codes of the next half
-                place(k_dst + (uint32_t)st * S::STAGE + (uint32_t)(STEP_K * x) * 1024u + swizzle, raw[x]);
-                raw[x] = fetch_v(v_page, x);
-            }
+            for (int x = 0; x < UNITS; ++x) place(k_dst + (uint32_t)k_stage * S::STAGE + (uint32_t)(STEP_K * x) * 1024u + swizzle, raw_k[x]);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            arrive(K_FULL + st);
-            const int after = page_of(i + 2);
-            sc = scales_of(next);
-            wait(V_EMPTY + st, parity);
-            if (key0 < j.from || key0 + KT > hi || __any_sync(0xFFFFFFFFu, now < 0)) {  // values of keys that do not count are zeros
+            arrive(K_FULL + k_stage);
+            if (++k_stage == S::NK) k_stage = 0, k_phase ^= 1u;
+        };
+        auto put_v = [&](int i, int ids) {
+            const int key0 = (j.kv0 + i) * KT;
+            wait(V_EMPTY + v_stage, v_phase);
+            if (key0 < j.from || key0 + KT > hi || __any_sync(0xFFFFFFFFu, ids < 0)) {  // values of keys that do not count are zeros
+                const int v_id = __shfl_sync(0xFFFFFFFFu, ids, v_group);
                 uint32_t keep[4] = {};
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
@@ -401,85 +495,42 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
                     if (v_id >= 0 && key >= j.from && key < hi) keep[e >> 2] |= 0xFFu << (8 * (e & 3));
                 }
 #pragma unroll
-                for (int x = 0; x < UNITS; ++x) raw[x].x &= keep[0], raw[x].y &= keep[1], raw[x].z &= keep[2], raw[x].w &= keep[3];
+                for (int x = 0; x < UNITS; ++x) raw_v[x].x &= keep[0], raw_v[x].y &= keep[1], raw_v[x].z &= keep[2], raw_v[x].w &= keep[3];
             }
 #pragma unroll
-            for (int x = 0; x < UNITS; ++x) {
-                place(v_dst + (uint32_t)st * S::STAGE + (uint32_t)(STEP_V * x) * 1024u + swizzle, raw[x]);
-                raw[x] = fetch_k(next, x);
-            }
+            for (int x = 0; x < UNITS; ++x) place(v_dst + (uint32_t)v_stage * S::STAGE + (uint32_t)(STEP_V * x) * 1024u + swizzle, raw_v[x]);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            arrive(V_FULL + st);
-            now = next, next = after;
-        }
-    } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
-        if (warp == MMA_WARP && lane == 0) {
-            // ---------------------------------------------------------------- MMA issue
-            auto scores = [&](int t, int it) {
-                const int st = it & 1;
-                const uint32_t d = tmem + S::COL_S + (uint32_t)(t * KT);
-                const uint64_t k0 = smc_tc_desc_sw128(sbase + S::OFF_K + (uint32_t)st * S::STAGE), q0 = smc_tc_desc_sw128(sbase + (uint32_t)t * S::Q_TILE);
-#pragma unroll
-                for (int p = S::PLANES - 1; p >= 0; --p)  // smallest products first
-#pragma unroll
-                    for (int ks = 0; ks < HD / 16; ++ks)
-                        smc_tc_mma(d, q0 + (uint64_t)(((uint32_t)p * S::Q_PLANE + (uint32_t)(ks >> 2) * S::SUB_Q + (uint32_t)(ks & 3) * 32u) >> 4),
-                                   k0 + (uint64_t)(((uint32_t)(ks >> 2) * (uint32_t)(KT * 128) + (uint32_t)(ks & 3) * 32u) >> 4), idesc_f16(KT), p < S::PLANES - 1 || ks > 0);
-                smc_tc_commit(bar(S_FULL + t));
-            };
-            auto outputs = [&](int t, int it) {
-                const int st = it & 1;
-                const uint32_t d = tmem + S::COL_O + (uint32_t)(t * HD), a = tmem + S::COL_S + (uint32_t)(t * KT);
-                const uint64_t v0 = smc_tc_desc_sw128(sbase + S::OFF_V + (uint32_t)st * S::STAGE);
-#pragma unroll
-                for (int p = S::PLANES - 1; p >= 0; --p)
-#pragma unroll
-                    for (int kk = 0; kk < KT / 16; ++kk)
-                        mma_ta(d, a + (uint32_t)(p * KT / 2 + kk * 8), v0 + (uint64_t)(((uint32_t)(kk >> 2) * (uint32_t)(HD * 128) + (uint32_t)(kk & 3) * 32u) >> 4), idesc_f16(HD),
-                               it > 0 || p < S::PLANES - 1 || kk > 0);
-            };
-            const int n0 = stop0 - j.i0, n1 = stop1 - j.i0, n = j.i1 - j.i0;  // (n0 <= n; n1 is n or 0)
-            smc_tc_wait(bar(K_FULL), 0u, abort_flag, status);
-            if (n0 > 0) {
-                smc_tc_wait(bar(Q_FULL), 0u, abort_flag, status);
-                smc_tc_fence_after();
-                scores(0, 0);
-            }
-            if (n1 > 0) {
-                smc_tc_wait(bar(Q_FULL + 1), 0u, abort_flag, status);
-                smc_tc_fence_after();
-                scores(1, 0);
-            }
-            smc_tc_commit(bar(K_EMPTY));
+            arrive(V_FULL + v_stage);
+            if (++v_stage == S::NV) v_stage = 0, v_phase ^= 1u;
+        };
+        next_k(id_k);
+        next_v(id_k);
+        id_v = id_k, id_next = page_of(j.i0 + 1);
+        put_k(0, id_k);
+        sc = scales_of(id_next);
+        next_k(id_next);
+        id_k = page_of(j.i0 + 2);
+        if (j.i0 + 1 < j.i1) put_k(1, id_next);
+        sc = scales_of(id_k);
+        next_k(id_k);
 #pragma unroll 1
-            for (int it = 0; it < n; ++it) {
-                const int st = it & 1, nx = (it + 1) & 1;
-                smc_tc_wait(bar(V_FULL + st), (uint32_t)(it >> 1) & 1u, abort_flag, status);
-                if (it < n0) {
-                    smc_tc_wait(bar(P_FULL), (uint32_t)it & 1u, abort_flag, status);
-                    smc_tc_fence_after();
-                    outputs(0, it);
-                    if (it + 1 == n0) smc_tc_commit(bar(O_FULL));
-                }
-                if (it + 1 < n) {
-                    smc_tc_wait(bar(K_FULL + nx), (uint32_t)((it + 1) >> 1) & 1u, abort_flag, status);
-                    smc_tc_fence_after();
-                    if (it + 1 < n0) scores(0, it + 1);
-                }
-                if (it < n1) {
-                    smc_tc_wait(bar(P_FULL + 1), (uint32_t)it & 1u, abort_flag, status);
-                    smc_tc_fence_after();
-                    outputs(1, it);
-                    if (it + 1 == n1) smc_tc_commit(bar(O_FULL + 1));
-                    if (it + 1 < n1) scores(1, it + 1);
-                }
-                smc_tc_commit(bar(V_EMPTY + st));
-                if (it + 1 < n) smc_tc_commit(bar(K_EMPTY + nx));
-            }
+        for (int i = j.i0; i < j.i1; ++i) {
+            put_v(i, id_v);
+            next_v(id_next);
+            const int after = page_of(i + 3);
+            id_v = id_next, id_next = id_k;
+            if (i + 2 < j.i1) put_k(i + 2 - j.i0, id_k);
+            id_k = after;
+            sc = scales_of(id_k);
+            next_k(id_k);
         }
-        __syncwarp();
+    } else if (lane == 0) {
+        // ---------------------------------------------------------------- MMA issue
+        const int n = j.i1 - j.i0;
+        if (warp == MMA_WARP) issue_mmas<HD, SPLIT, 0>(sbase, stop0 - j.i0, n, bar(0), abort_flag, status);
+        else if (two) issue_mmas<HD, SPLIT, 1>(sbase, stop1 - j.i0, n, bar(0), abort_flag, status);
     }
+    __syncwarp();
     smc_tc_fence_before();
     __syncthreads();
     if (warp == MMA_WARP) {
@@ -493,10 +544,10 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(256) paged_prompt_join_kernel(const smc_paged_view c, const smc_paged_query u, int items, int split, const float *__restrict__ work)
 {
     smc_grid_dep_sync();
-    constexpr int KT = Shape<HD, sizeof(T) == 4>::KT, E = HD / 32;
+    constexpr int E = HD / 32;
     const int lane = threadIdx.x & 31, b = blockIdx.x / (PAIRS / 8), m = blockIdx.x % (PAIRS / 8) * 8 + (threadIdx.x >> 5);
     Job j;
-    if (!job_of<KT>(c, u, items - 1 - b / c.kvh, b % c.kvh, 0, split, j, nullptr) || j.pieces == 1 || m >= j.pairs) return;
+    if (!job_of(c, u, items - 1 - b / c.kvh, b % c.kvh, 0, split, j, nullptr) || j.pieces == 1 || m >= j.pairs) return;
     const float *row = work + ((size_t)b * split * PAIRS + m) * (HD + 4);
     const size_t step = (size_t)PAIRS * (HD + 4);
     float top = -INFINITY, sum = 0.0f, o[E] = {};

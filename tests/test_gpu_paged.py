@@ -283,6 +283,25 @@ def test_a_run_of_them_together(cuda, dtype):
             lens = [n - 2 for n in lens]
 
 
+@pytest.mark.parametrize("dtype,heads,dim", [(F32, 16, 128), (BF16, 16, 128), (F32, 8, 64), (BF16, 8, 64)])
+def test_prompts_back_to_back(cuda, dtype, heads, dim):
+    """Two lengths in turn without a pause, every CTA's steps many: each result has its own bits again and again, and no wait is given up."""
+    p = Pair(cuda, [1500, 1100], kvh=4, dim=dim, page=64)
+    p.fill([1500, 1100])
+    q = randn((777, heads, dim), "back", heads).to(dtype).cuda()
+    calls = [([777, 0], [777, 1100]), ([500, 277], [1500, 900])]
+    first = []
+    for i in range(40):
+        rows, lens = calls[i % 2]
+        got = p.cache.attention(q, p.dtable, ints(lens), dim ** -0.5, row_start=starts(rows), max_rows=max(rows))
+        if i < 2:
+            near(got, q.cpu(), p, lens, rows, dim ** -0.5)
+            first.append(got)
+        else:
+            assert torch.equal(got, first[i % 2])
+    assert cuda.device_status() == 0
+
+
 # ---- where and when it runs
 @pytest.mark.parametrize("rows", [1, 3, 140])
 def test_captured_calls_serve_what_the_arrays_hold(cuda, rows):
