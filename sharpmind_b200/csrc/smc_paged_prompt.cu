@@ -21,16 +21,16 @@ constexpr float R_ABOVE = 15.0f, R_BELOW = 8.0f;
 
 // A wait names a phase by its parity: no barrier passes a phase before its waiter has seen the one before.  (PV_DONE may for a softmax, which looks
 // at it only in step i for the product of step i - 1, where neither the one before can be missing nor the one after be there.)
-enum { K_FULL = 0, K_EMPTY = 4, V_FULL = 8, V_EMPTY = 12, S_FULL = 16, P_FULL = 20 /* [tile][step parity] */, PV_DONE = 24, Q_FULL = 26, O_FULL = 28, BARS = 30 };
+enum { FULL = 0, EMPTY = 4, S_FULL = 8, P_FULL = 12 /* [tile][step parity] */, PV_DONE = 16, Q_FULL = 18, O_FULL = 20, BARS = 22 };
 
 template <int HD, bool SPLIT>
 struct Shape {
-    static constexpr int PLANES = SPLIT ? 2 : 1, NK = 4, NV = SPLIT ? 2 : 4;
+    static constexpr int PLANES = SPLIT ? 2 : 1, STAGES = SPLIT ? 2 : 4;
     static constexpr uint32_t SUB_Q = TILE * 128, Q_PLANE = HD / 64 * SUB_Q, Q_TILE = PLANES * Q_PLANE;
-    static constexpr uint32_t STAGE = KT * HD * 2;  // fp16 keys or values of a step
-    static constexpr uint32_t OFF_K = 2 * Q_TILE, OFF_V = OFF_K + NK * STAGE, OFF_SC = OFF_V + NV * STAGE, OFF_BAR = OFF_SC + SC_SLOTS * G * 16, SMEM = OFF_BAR + 256;
+    static constexpr uint32_t HALF = KT * HD * 2, STAGE = 2 * HALF;  // fp16 keys of a step, values of the last step but one
+    static constexpr uint32_t OFF_K = 2 * Q_TILE, OFF_SC = OFF_K + STAGES * STAGE, OFF_BAR = OFF_SC + SC_SLOTS * G * 16, SMEM = OFF_BAR + 256;
     static constexpr uint32_t COL_S = 0, COL_O = 4 * KT, COLS = 512;  // scores [tile][step parity]
-    static_assert(BARS * 8 + 8 <= 256 && SMEM <= 227 * 1024 && COL_O + 2 * HD <= COLS && NK < SC_SLOTS, "");
+    static_assert(BARS * 8 + 8 <= 256 && SMEM <= 227 * 1024 && COL_O + 2 * HD <= COLS && STAGES + 2 < SC_SLOTS, "");
 };
 // tcgen05.mma whose operands are known at compile time, up to the shared memory's base: operands that come through registers take an issuing
 // thread some 140 clocks an MMA (measured here), these less than the MMA itself.  D, A_COL: columns of tensor memory, all of which is the CTA's, so it starts
@@ -107,64 +107,48 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b)
 }
 __host__ __device__ constexpr uint32_t idesc_f16(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TILE >> 4) << 24); }
 
-// One thread issues a tile's MMAs: scores of two steps ahead; then, step by step, O += P(i) V(i) and the scores of step i + 2, which take the buffer that P(i) was
-// in.  The wait for that product delays nobody: the softmax has step i + 1 meanwhile, and the tensor cores the other tile's MMAs.
+// One thread issues a tile's MMAs: at step x, O += P(x - 2) V(x - 2) and the scores of x.  These take the columns that P(x - 2) is in: the MMAs of a thread run in
+// their order (checked: weights overwritten by the next product's scores at once, 30 000 times).
 template <int HD, bool SPLIT, int TILE_NO>
 __device__ __forceinline__ void issue_mmas(uint32_t sbase, int mine, int n, uint32_t bars, volatile uint32_t *abort_flag, int *status)
 {
     using S = Shape<HD, SPLIT>;
-    constexpr int UNROLL = S::NK;  // stages are constants
-    static_assert(S::NK % 2 == 0 && S::NK % S::NV == 0, "");
+    static_assert(S::STAGES % 2 == 0, "");
     const uint32_t base = ((sbase >> 4) & 0x3FFFu) | (1u << 16);
-    auto wait = [&](int i, uint32_t parity) { smc_tc_wait(bars + 8u * (uint32_t)i, parity & 1u, abort_flag, status); };
-    auto scores = [&](auto stage, int it) {  // it % NK = stage
-        constexpr int st = decltype(stage)::v;
-        wait(K_FULL + st, (uint32_t)(it / S::NK));
-        if (it >= mine) {  // the other tile goes on
-            smc_mbar_arrive(bars + 8u * (K_EMPTY + st));
-            return;
-        }
+    auto bar = [&](int i) { return bars + 8u * (uint32_t)i; };
+    auto wait = [&](int i, uint32_t parity) { smc_tc_wait(bar(i), parity & 1u, abort_flag, status); };
+    bool there = false;  // the next stage, as far as is known
+    auto step = [&](auto stage, int x) {  // x % STAGES = stage
+        constexpr int st = decltype(stage)::v, next = (st + 1) % S::STAGES;
+        if (!there) wait(FULL + st, (uint32_t)(x / S::STAGES));
+        if (x >= 2 && x - 2 < mine) wait(P_FULL + 2 * TILE_NO + st % 2, (uint32_t)((x - 2) >> 1));
         smc_tc_fence_after();
-        each<S::PLANES * (HD / 16)>([&](auto x) {
-            constexpr int p = S::PLANES - 1 - decltype(x)::v / (HD / 16), ks = decltype(x)::v % (HD / 16);  // smallest products first
-            mma_ss<S::COL_S + (2 * TILE_NO + st % 2) * KT, TILE_NO * S::Q_TILE + p * S::Q_PLANE + ks / 4 * S::SUB_Q + ks % 4 * 32,
-                   S::OFF_K + st * S::STAGE + ks / 4 * (KT * 128) + ks % 4 * 32, idesc_f16(KT)>(base, decltype(x)::v > 0);
-        });
-        smc_tc_commit(bars + 8u * (S_FULL + 2 * TILE_NO + st % 2));
-        smc_tc_commit(bars + 8u * (K_EMPTY + st));
-    };
-    auto outputs = [&](auto stage, int it) {
-        constexpr int st = decltype(stage)::v, vs = st % S::NV;
-        wait(V_FULL + vs, (uint32_t)(it / S::NV));
-        if (it >= mine) {
-            smc_mbar_arrive(bars + 8u * (V_EMPTY + vs));
-            return;
+        there = smc_mbar_test(bar(FULL + next), (uint32_t)((x + 1) / S::STAGES) & 1u);
+        if (x >= 2 && x - 2 < mine) {
+            each<S::PLANES * (KT / 16)>([&](auto i) {
+                constexpr int p = S::PLANES - 1 - decltype(i)::v / (KT / 16), kk = decltype(i)::v % (KT / 16);  // smallest products first
+                mma_ts<S::COL_O + TILE_NO * HD, S::COL_S + (2 * TILE_NO + st % 2) * KT + p * (KT / 2) + kk * 8, S::OFF_K + st * S::STAGE + S::HALF + kk * 32, idesc_f16(HD)>(
+                    base, decltype(i)::v > 0 || x > 2);
+            });
+            smc_tc_commit(bar(PV_DONE + TILE_NO));
+            if (x - 1 == mine) smc_tc_commit(bar(O_FULL + TILE_NO));
         }
-        wait(P_FULL + 2 * TILE_NO + st % 2, (uint32_t)(it >> 1));
-        smc_tc_fence_after();
-        each<S::PLANES * (KT / 16)>([&](auto x) {
-            constexpr int p = S::PLANES - 1 - decltype(x)::v / (KT / 16), kk = decltype(x)::v % (KT / 16);
-            mma_ts<S::COL_O + TILE_NO * HD, S::COL_S + (2 * TILE_NO + st % 2) * KT + p * (KT / 2) + kk * 8, S::OFF_V + vs * S::STAGE + kk * 32, idesc_f16(HD)>(
-                base, decltype(x)::v > 0 || it > 0);
-        });
-        smc_tc_commit(bars + 8u * (PV_DONE + TILE_NO));
-        if (it + 1 == mine) smc_tc_commit(bars + 8u * (O_FULL + TILE_NO));
-        smc_tc_commit(bars + 8u * (V_EMPTY + vs));
+        if (x < mine) {
+            each<S::PLANES * (HD / 16)>([&](auto i) {
+                constexpr int p = S::PLANES - 1 - decltype(i)::v / (HD / 16), ks = decltype(i)::v % (HD / 16);
+                mma_ss<S::COL_S + (2 * TILE_NO + st % 2) * KT, TILE_NO * S::Q_TILE + p * S::Q_PLANE + ks / 4 * S::SUB_Q + ks % 4 * 32,
+                       S::OFF_K + st * S::STAGE + ks / 4 * (KT * 128) + ks % 4 * 32, idesc_f16(KT)>(base, decltype(i)::v > 0);
+            });
+            smc_tc_commit(bar(S_FULL + 2 * TILE_NO + st % 2));
+        }
+        if (x < mine + 2 && mine > 0) smc_tc_commit(bar(EMPTY + st));
+        else smc_mbar_arrive(bar(EMPTY + st));  // the other tile goes on
     };
     if (mine > 0) wait(Q_FULL + TILE_NO, 0u);
-    scores(ic<0>(), 0);
-    if (n > 1) scores(ic<1>(), 1);
 #pragma unroll 1
-    for (int it = 0; it < n; it += UNROLL)
-        each<UNROLL>([&](auto x) {
-            constexpr int st = decltype(x)::v;
-            const int i = it + st;
-            if (i >= n) return;
-            outputs(x, i);
-            if (i + 2 < n) {
-                if (i + 2 < mine) wait(PV_DONE + TILE_NO, (uint32_t)i);
-                scores(ic<(st + 2) % UNROLL>(), i + 2);
-            }
+    for (int x0 = 0; x0 < n + 2; x0 += S::STAGES)
+        each<S::STAGES>([&](auto i) {
+            if (x0 + decltype(i)::v < n + 2) step(i, x0 + decltype(i)::v);
         });
 }
 
@@ -233,8 +217,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
     }
     if (threadIdx.x == 0) {
         const uint32_t readers = j.pairs > TILE ? 2u : 1u;
-        for (int i = 0; i < S::NK; ++i) smc_mbar_init(bar(K_FULL + i), 4), smc_mbar_init(bar(K_EMPTY + i), readers);
-        for (int i = 0; i < S::NV; ++i) smc_mbar_init(bar(V_FULL + i), 4), smc_mbar_init(bar(V_EMPTY + i), readers);
+        for (int i = 0; i < S::STAGES; ++i) smc_mbar_init(bar(FULL + i), 4), smc_mbar_init(bar(EMPTY + i), readers);
         for (int i = 0; i < 4; ++i) smc_mbar_init(bar(S_FULL + i), 1), smc_mbar_init(bar(P_FULL + i), 4);
         for (int i = 0; i < 2; ++i) smc_mbar_init(bar(PV_DONE + i), 1), smc_mbar_init(bar(O_FULL + i), 1), smc_mbar_init(bar(Q_FULL + i), 4);
         *abort_flag = 0;
@@ -298,11 +281,12 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
         }
         // rows of this tile: [lowest, highest] positions, for tiles that every row sees whole
         const int lowest = j.len - j.n_rows + (j.m0 + t * TILE) / group, highest = j.len - j.n_rows + (j.m0 + min(j.pairs, (t + 1) * TILE) - 1) / group;
+        bool there = false;  // the next scores, as far as is known
 #pragma unroll 1
         for (int i = j.i0; i < stop; ++i) {
             const int it = i - j.i0, key0 = (j.kv0 + i) * KT;
             const uint32_t col_s = col_s0 + (uint32_t)((it & 1) * KT);
-            wait(S_FULL + 2 * t + (it & 1), (uint32_t)(it >> 1));
+            if (!there) wait(S_FULL + 2 * t + (it & 1), (uint32_t)(it >> 1));
             smc_tc_fence_after();
             uint32_t s[KT];
 #pragma unroll
@@ -363,6 +347,8 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
                 }
             }
             const float ref = R == -INFINITY ? 0.0f : R;
+            // (asked here, the answer is there when this step is done)
+            there = i + 1 < stop && __all_sync(0xFFFFFFFFu, smc_mbar_test(bar(S_FULL + 2 * t + ((it + 1) & 1)), (uint32_t)((it + 1) >> 1) & 1u));
             uint32_t rest[SPLIT ? KT / 2 : 1];
 #pragma unroll
             for (int k = 0; k < G; ++k) {
@@ -430,7 +416,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
         const uint8_t *k_base = c.k + ((size_t)j.h * HD << c.shift) + 64 * (w % IN_K) + 16 * q4, *v_base = c.v + ((size_t)j.h * HD << c.shift) + ((size_t)(8 * (w / IN_V) + r8) << c.shift);
         const int v_group = 4 * (w % IN_V) + q4;
         const uint32_t swizzle = (uint32_t)(r8 * 128 + ((2 * q4) ^ r8) * 16), flip = (uint32_t)((2 * q4 ^ r8) * 16) ^ (uint32_t)(((2 * q4 + 1) ^ r8) * 16);
-        const uint32_t k_dst = sbase + S::OFF_K + (uint32_t)((w % IN_K) * KT * 128 + w / IN_K * 1024), v_dst = sbase + S::OFF_V + (uint32_t)((w % IN_V) * HD * 128 + w / IN_V * 1024);
+        const uint32_t k_dst = sbase + S::OFF_K + (uint32_t)((w % IN_K) * KT * 128 + w / IN_K * 1024), v_dst = sbase + S::OFF_K + S::HALF + (uint32_t)((w % IN_V) * HD * 128 + w / IN_V * 1024);
         // Page of this lane's group of 16 keys (lane % G) of tile i, or -1.  Codes of page 0 stand in for those of a page that is not there: nothing of a
         // key that no row sees reaches a result, and undefined codes among the values are made zeros below.
         auto page_of = [&](int i) {
@@ -454,75 +440,53 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
             sts128(at, h[0], h[1], h[2], h[3]);
             sts128(at ^ flip, h[4], h[5], h[6], h[7]);
         };
-        // keys two steps ahead of the values, as the MMAs want them; codes of the next step of each are on their way meanwhile
+        // step x brings the keys of x and the values of x - 2; codes of the next step of each are on their way meanwhile
+        const int n = j.i1 - j.i0;
         uint4 raw_k[UNITS], raw_v[UNITS];
-        int id_v, id_next, id_k = page_of(j.i0);  // pages of the next values, of those after, and of the next keys
+        int id_k = page_of(j.i0), id_1 = -1, id_v = -1;  // pages of the keys of step x, of those before, of the values
         float2 sc = scales_of(id_k);
-        auto next_k = [&](int ids) {
 #pragma unroll
-            for (int x = 0; x < UNITS; ++x) raw_k[x] = fetch_k(ids, x);
-        };
-        auto next_v = [&](int ids) {
-            const uint8_t *v_page = v_base + (size_t)(uint32_t)max(__shfl_sync(0xFFFFFFFFu, ids, v_group), 0) * stride + ((16 * v_group) & (page - 1));
+        for (int i = 0; i < UNITS; ++i) raw_k[i] = fetch_k(id_k, i);
+#pragma unroll 1
+        for (int x = 0; x < n + 2; ++x) {
+            const int st = x % S::STAGES, id_next = page_of(j.i0 + x + 1);
+            wait(EMPTY + st, (uint32_t)(x / S::STAGES) ^ 1u);  // (a fresh barrier passes the first)
+            if (x >= 2) {
+                const int key0 = (j.kv0 + j.i0 + x - 2) * KT;
+                if (key0 < j.from || key0 + KT > hi || __any_sync(0xFFFFFFFFu, id_v < 0)) {  // values of keys that do not count are zeros
+                    const int v_id = __shfl_sync(0xFFFFFFFFu, id_v, v_group);
+                    uint32_t keep[4] = {};
 #pragma unroll
-            for (int x = 0; x < UNITS; ++x) raw_v[x] = fetch_v(v_page, x);
-        };
-        int k_stage = 0, v_stage = 0;
-        uint32_t k_phase = 1, v_phase = 1;  // (a fresh barrier passes the first)
-        auto put_k = [&](int it, int ids) {
-            wait(K_EMPTY + k_stage, k_phase);
-            if (w == 0 && lane < G) {
-                // scale of keys; log2 and reciprocal of that of values (a power of two's exponent).  An undefined one of either makes the second undefined
-                const float both = sc.x + sc.y, e = (float)((int)(__float_as_uint(sc.y) >> 23) - 127);
-                reinterpret_cast<float4 *>(smem + S::OFF_SC)[(it % SC_SLOTS) * G + lane] =
-                    ids < 0 ? make_float4(0.0f, -INFINITY, 0.0f, 0.0f) : make_float4(sc.x, both == both ? e : both, 1.0f / sc.y, 0.0f);
-            }
+                    for (int e = 0; e < 16; ++e) {
+                        const int key = key0 + 16 * v_group + e;
+                        if (v_id >= 0 && key >= j.from && key < hi) keep[e >> 2] |= 0xFFu << (8 * (e & 3));
+                    }
 #pragma unroll
-            for (int x = 0; x < UNITS; ++x) place(k_dst + (uint32_t)k_stage * S::STAGE + (uint32_t)(STEP_K * x) * 1024u + swizzle, raw_k[x]);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            arrive(K_FULL + k_stage);
-            if (++k_stage == S::NK) k_stage = 0, k_phase ^= 1u;
-        };
-        auto put_v = [&](int i, int ids) {
-            const int key0 = (j.kv0 + i) * KT;
-            wait(V_EMPTY + v_stage, v_phase);
-            if (key0 < j.from || key0 + KT > hi || __any_sync(0xFFFFFFFFu, ids < 0)) {  // values of keys that do not count are zeros
-                const int v_id = __shfl_sync(0xFFFFFFFFu, ids, v_group);
-                uint32_t keep[4] = {};
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int key = key0 + 16 * v_group + e;
-                    if (v_id >= 0 && key >= j.from && key < hi) keep[e >> 2] |= 0xFFu << (8 * (e & 3));
+                    for (int i = 0; i < UNITS; ++i) raw_v[i].x &= keep[0], raw_v[i].y &= keep[1], raw_v[i].z &= keep[2], raw_v[i].w &= keep[3];
                 }
 #pragma unroll
-                for (int x = 0; x < UNITS; ++x) raw_v[x].x &= keep[0], raw_v[x].y &= keep[1], raw_v[x].z &= keep[2], raw_v[x].w &= keep[3];
+                for (int i = 0; i < UNITS; ++i) place(v_dst + (uint32_t)st * S::STAGE + (uint32_t)(STEP_V * i) * 1024u + swizzle, raw_v[i]);
             }
+            id_v = id_1, id_1 = id_k;
+            const uint8_t *v_page = v_base + (size_t)(uint32_t)max(__shfl_sync(0xFFFFFFFFu, id_v, v_group), 0) * stride + ((16 * v_group) & (page - 1));
 #pragma unroll
-            for (int x = 0; x < UNITS; ++x) place(v_dst + (uint32_t)v_stage * S::STAGE + (uint32_t)(STEP_V * x) * 1024u + swizzle, raw_v[x]);
+            for (int i = 0; i < UNITS; ++i) raw_v[i] = fetch_v(v_page, i);
+            if (x < n) {
+                if (w == 0 && lane < G) {
+                    // scale of keys; log2 and reciprocal of that of values (a power of two's exponent).  An undefined one of either makes the second undefined
+                    const float both = sc.x + sc.y, e = (float)((int)(__float_as_uint(sc.y) >> 23) - 127);
+                    reinterpret_cast<float4 *>(smem + S::OFF_SC)[(x % SC_SLOTS) * G + lane] =
+                        id_k < 0 ? make_float4(0.0f, -INFINITY, 0.0f, 0.0f) : make_float4(sc.x, both == both ? e : both, 1.0f / sc.y, 0.0f);
+                }
+#pragma unroll
+                for (int i = 0; i < UNITS; ++i) place(k_dst + (uint32_t)st * S::STAGE + (uint32_t)(STEP_K * i) * 1024u + swizzle, raw_k[i]);
+            }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            arrive(V_FULL + v_stage);
-            if (++v_stage == S::NV) v_stage = 0, v_phase ^= 1u;
-        };
-        next_k(id_k);
-        next_v(id_k);
-        id_v = id_k, id_next = page_of(j.i0 + 1);
-        put_k(0, id_k);
-        sc = scales_of(id_next);
-        next_k(id_next);
-        id_k = page_of(j.i0 + 2);
-        if (j.i0 + 1 < j.i1) put_k(1, id_next);
-        sc = scales_of(id_k);
-        next_k(id_k);
-#pragma unroll 1
-        for (int i = j.i0; i < j.i1; ++i) {
-            put_v(i, id_v);
-            next_v(id_next);
-            const int after = page_of(i + 3);
-            id_v = id_next, id_next = id_k;
-            if (i + 2 < j.i1) put_k(i + 2 - j.i0, id_k);
-            id_k = after;
+            arrive(FULL + st);
+            id_k = id_next;
             sc = scales_of(id_k);
-            next_k(id_k);
+#pragma unroll
+            for (int i = 0; i < UNITS; ++i) raw_k[i] = fetch_k(id_k, i);
         }
     } else if (lane == 0) {
         // ---------------------------------------------------------------- MMA issue
