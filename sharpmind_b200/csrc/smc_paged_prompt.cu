@@ -6,8 +6,8 @@
 //   bfloat16  queries exact in fp16 after a power of two per row, weights rounded to 11 bits
 //   fp32      queries and weights as hi + lo, 22 bits, two products each
 // With the pages' scales, constant over 16 keys:  y = S f + b, f = s_k * row factor, b = log2(s_v);  w = 2^(y - R);  l = sum w / s_v;  out = O / l.
-// R follows the running maximum of y only where that gets more than 2^15 above it (then to 2^8 below), so O, in tensor memory, is rarely
-// multiplied again; a weight stays under 2^15 and counts down to 2^-24.
+// R is 6 below the maximum of y of a row's first step and goes up (to 6 below the maximum) only where a step's weights sum up to more than fp16 holds: a step takes
+// no maximum, and O, in tensor memory, is rarely multiplied again.  A weight counts down to 2^-24, 2^-30 of the largest of the first step.
 // Warp roles:  0 .. 3, 4 .. 7  softmax of tile 0, 1      8 .. 11  codes to fp16      12, 13  MMA issue of tile 0, 1
 // Scores have two buffers a tile, so a softmax finds its next ones there.
 // Few pairs: the steps are split over CTAs, whose partial results a second kernel joins.
@@ -17,7 +17,7 @@
 namespace {
 
 constexpr int PAIRS = 256, TILE = 128, KT = 64, G = KT / 16, SOFT_WARPS = 8, CONV_WARP = 8, MMA_WARP = 12, THREADS = 32 * (MMA_WARP + 2), SC_SLOTS = 8;
-constexpr float R_ABOVE = 15.0f, R_BELOW = 8.0f;
+constexpr float R_BELOW = 6.0f, SUM_MOST = 65000.0f;
 
 // A wait names a phase by its parity: no barrier passes a phase before its waiter has seen the one before.  (PV_DONE may for a softmax, which looks
 // at it only in step i for the product of step i - 1, where neither the one before can be missing nor the one after be there.)
@@ -73,6 +73,12 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r)
         "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
+                 "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w)
 {
@@ -105,6 +111,8 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b)
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
+// power of two that brings a row's largest magnitude to [2^14, 2^15)
+__device__ __forceinline__ int row_shift(float most) { return min(14 - ((int)(__float_as_uint(most) >> 23) - 127), 126); }
 __host__ __device__ constexpr uint32_t idesc_f16(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TILE >> 4) << 24); }
 
 // One thread issues a tile's MMAs: at step x, O += P(x - 2) V(x - 2) and the scores of x.  These take the columns that P(x - 2) is in: the MMAs of a thread run in
@@ -239,43 +247,48 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
     if (warp < SOFT_WARPS) {
         const int t = warp >> 2, rl = 32 * (warp & 3) + lane, m = t * TILE + rl, stop = t ? stop1 : stop0;
         const bool real = m < j.pairs;
-        const int pair = j.m0 + (real ? m : 0), tok = pair / group, head = j.h * group + pair - tok * group;
+        const int pair = j.m0 + (real ? m : 0), tok = pair / group;
         const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16), col_s0 = lanes + S::COL_S + (uint32_t)(2 * t * KT), col_o = lanes + S::COL_O + (uint32_t)(t * HD);
         const int pos = j.len - j.n_rows + tok;
         float rowf = 0.0f, R = -INFINITY, l = 0.0f;
         if (stop > j.i0) {
-            const T *src = static_cast<const T *>(u.q) + (long long)(j.r0 + tok) * u.q_stride + (size_t)head * HD;
-            float most = 0.0f;
-#pragma unroll 8
-            for (int e = 0; e < HD; e += 4) {
-                float v[4];
-                smc_paged_load4(src + e, v);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) most = fmaxf(most, fabsf(v[k]));
-            }
-            // the largest magnitude of the row goes to [2^14, 2^15); a negative scale turns the queries' sign
-            const int up = min(14 - ((int)(__float_as_uint(most) >> 23) - 127), 126);
-            float fac = __uint_as_float((uint32_t)(up + 127) << 23);
-            rowf = fabsf(u.scale) * 1.44269504088896341f * __uint_as_float((uint32_t)(127 - up) << 23);
-            if (u.scale < 0.0f) fac = -fac;
-            if (!real) fac = 0.0f;
+            // the warp's 32 rows, 16 bytes a lane, the lanes of a row side by side
+            constexpr int N = 16 / (int)sizeof(T), LANES = HD / N, AT_ONCE = 32 / LANES;
+            const int e = lane % LANES * N, sub = lane / LANES;
+            float mine = 0.0f;  // the largest magnitude of this lane's own row
 #pragma unroll 4
-            for (int e = 0; e < HD; e += 8) {
-                float v[8], a[4], b[4];
-                smc_paged_load4(src + e, a), smc_paged_load4(src + e + 4, b);
+            for (int r = 0; r < 32; r += AT_ONCE) {
+                const int row = 32 * (warp & 3) + r + sub, at = t * TILE + row, pr = j.m0 + (at < j.pairs ? at : 0), tk = pr / group;
+                const T *src = static_cast<const T *>(u.q) + (long long)(j.r0 + tk) * u.q_stride + (size_t)(j.h * group + pr - tk * group) * HD + e;
+                float v[N], most = 0.0f;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] = a[k] * fac, v[4 + k] = b[k] * fac;
-                uint32_t hi[4], lo[4];
+                for (int k = 0; k < N; k += 4) smc_paged_load4(src + k, *reinterpret_cast<float(*)[4]>(v + k));
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    hi[k] = half2_bits(v[2 * k], v[2 * k + 1]);
-                    if (SPLIT) lo[k] = rest_bits(v[2 * k], v[2 * k + 1], hi[k]);
+                for (int k = 0; k < N; ++k) most = fmaxf(most, fabsf(v[k]));
+#pragma unroll
+                for (int o = LANES / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
+                const float theirs = __shfl_sync(0xFFFFFFFFu, most, (lane % AT_ONCE) * LANES);
+                if (lane / AT_ONCE * AT_ONCE == r) mine = theirs;
+                // the largest magnitude of the row goes to [2^14, 2^15); a negative scale turns the queries' sign
+                float fac = __uint_as_float((uint32_t)(row_shift(most) + 127) << 23);
+                if (u.scale < 0.0f) fac = -fac;
+                if (at >= j.pairs) fac = 0.0f;
+                uint32_t hi[N / 2], lo[N / 2];
+#pragma unroll
+                for (int k = 0; k < N / 2; ++k) {
+                    hi[k] = half2_bits(v[2 * k] * fac, v[2 * k + 1] * fac);
+                    if (SPLIT) lo[k] = rest_bits(v[2 * k] * fac, v[2 * k + 1] * fac, hi[k]);
                 }
-                const uint32_t at = sbase + (uint32_t)t * S::Q_TILE + (uint32_t)(e >> 6) * S::SUB_Q + (uint32_t)(rl >> 3) * 1024u + (uint32_t)(rl & 7) * 128u +
-                                    (uint32_t)((((e >> 3) & 7) ^ (rl & 7)) << 4);
-                sts128(at, hi[0], hi[1], hi[2], hi[3]);
-                if (SPLIT) sts128(at + S::Q_PLANE, lo[0], lo[1], lo[2], lo[3]);
+                const uint32_t dst = sbase + (uint32_t)t * S::Q_TILE + (uint32_t)(e >> 6) * S::SUB_Q + (uint32_t)(row >> 3) * 1024u + (uint32_t)(row & 7) * 128u +
+                                     (uint32_t)((((e >> 3) & 7) ^ (row & 7)) << 4);
+                if constexpr (SPLIT) {
+                    const uint32_t half = (uint32_t)(e & 4) * 2u;
+                    smc_sts64(dst + half, make_uint2(hi[0], hi[1])), smc_sts64(dst + S::Q_PLANE + half, make_uint2(lo[0], lo[1]));
+                } else {
+                    sts128(dst, hi[0], hi[1], hi[2], hi[3]);
+                }
             }
+            rowf = fabsf(u.scale) * 1.44269504088896341f * __uint_as_float((uint32_t)(127 - row_shift(mine)) << 23);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             arrive(Q_FULL + t);
         }
@@ -313,24 +326,54 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
                 return x;
             };
             float4 x[G];
-            float y[G];
 #pragma unroll
-            for (int k = 0; k < G; ++k) {
-                x[k] = scales(k);
-                float m4[4];
+            for (int k = 0; k < G; ++k) x[k] = scales(k);
+            // (asked here, the answer is there when this step is done)
+            there = i + 1 < stop && __all_sync(0xFFFFFFFFu, smc_mbar_test(bar(S_FULL + 2 * t + ((it + 1) & 1)), (uint32_t)((it + 1) >> 1) & 1u));
+            float add;
+#pragma unroll 1
+            for (bool again = true;;) {
+                const float ref = R == -INFINITY ? 0.0f : R;
+                float total = 0.0f;
+                add = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    m4[e] = fmaxf(fmaxf(__uint_as_float(s[16 * k + e]), __uint_as_float(s[16 * k + 4 + e])), fmaxf(__uint_as_float(s[16 * k + 8 + e]), __uint_as_float(s[16 * k + 12 + e])));
-                y[k] = fmaf(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), x[k].x, x[k].y);
-            }
-            const float top = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));  // (what is not a number a maximum drops)
-            float corr = 1.0f;
-            if (top > R + R_ABOVE) {
-                const float was = R;
-                R = top - R_BELOW;
-                corr = ex2(was - R);
-            }
-            if (__any_sync(0xFFFFFFFFu, corr != 1.0f)) {
+                for (int k = 0; k < G; ++k) {
+                    const float2 f = make_float2(x[k].x, x[k].x), bias = make_float2(x[k].y - ref, x[k].y - ref);
+                    float2 w[8];
+                    uint32_t p[8], rest[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        w[e] = fma2(make_float2(__uint_as_float(s[16 * k + 2 * e]), __uint_as_float(s[16 * k + 2 * e + 1])), f, bias);
+                        w[e].x = ex2(w[e].x), w[e].y = ex2(w[e].y);
+                        p[e] = half2_bits(w[e].x, w[e].y);
+                        if constexpr (SPLIT) rest[e] = rest_bits(w[e].x, w[e].y, p[e]);
+                    }
+                    tmem_st8(col_s + (uint32_t)(8 * k), p);
+                    if constexpr (SPLIT) tmem_st8(col_s + (uint32_t)(KT / 2 + 8 * k), rest);
+                    const float2 sum2 = add2(add2(add2(w[0], w[1]), add2(w[2], w[3])), add2(add2(w[4], w[5]), add2(w[6], w[7])));
+                    const float sum = sum2.x + sum2.y;
+                    total += sum, add = fmaf(sum, x[k].z, add);
+                }
+                // No maximum is taken where the weights' sum tells that none of them is too large.  (A row's first step has no R yet.)
+                const bool bad = again && (R == -INFINITY || total > SUM_MOST);
+                if (!__any_sync(0xFFFFFFFFu, bad)) break;
+                again = false;
+                tmem_wait_st();
+                float top = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < G; ++k) {
+                    float m4[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        m4[e] = fmaxf(fmaxf(__uint_as_float(s[16 * k + e]), __uint_as_float(s[16 * k + 4 + e])), fmaxf(__uint_as_float(s[16 * k + 8 + e]), __uint_as_float(s[16 * k + 12 + e])));
+                    top = fmaxf(top, fmaf(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), x[k].x, x[k].y));  // (what is not a number a maximum drops)
+                }
+                float corr = 1.0f;
+                if (bad && top > -INFINITY) {
+                    const float was = R;
+                    R = top - R_BELOW;
+                    corr = ex2(was - R);
+                }
                 l *= corr;
                 if (it > 0) {
                     wait(PV_DONE + t, (uint32_t)(it - 1));  // (the one before that: these scores waited for it)
@@ -346,33 +389,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
                     }
                 }
             }
-            const float ref = R == -INFINITY ? 0.0f : R;
-            // (asked here, the answer is there when this step is done)
-            there = i + 1 < stop && __all_sync(0xFFFFFFFFu, smc_mbar_test(bar(S_FULL + 2 * t + ((it + 1) & 1)), (uint32_t)((it + 1) >> 1) & 1u));
-            uint32_t rest[SPLIT ? KT / 2 : 1];
-#pragma unroll
-            for (int k = 0; k < G; ++k) {
-                const float2 f = make_float2(x[k].x, x[k].x), bias = make_float2(x[k].y - ref, x[k].y - ref);
-                float2 w[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    w[e] = fma2(make_float2(__uint_as_float(s[16 * k + 2 * e]), __uint_as_float(s[16 * k + 2 * e + 1])), f, bias);
-                    w[e].x = ex2(w[e].x), w[e].y = ex2(w[e].y);
-                }
-                const float2 sum = add2(add2(add2(w[0], w[1]), add2(w[2], w[3])), add2(add2(w[4], w[5]), add2(w[6], w[7])));
-                l = fmaf(sum.x + sum.y, x[k].z, l);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint32_t hi16 = half2_bits(w[e].x, w[e].y);
-                    if constexpr (SPLIT) rest[8 * k + e] = rest_bits(w[e].x, w[e].y, hi16);
-                    s[8 * k + e] = hi16;  // (the scores there are used up)
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < KT / 2; k += 16) {
-                tmem_st16(col_s + (uint32_t)k, s + k);
-                if constexpr (SPLIT) tmem_st16(col_s + (uint32_t)(KT / 2 + k), rest + k);
-            }
+            l += add;
             tmem_wait_st();
             smc_tc_fence_before();
             arrive(P_FULL + 2 * t + (it & 1));
@@ -380,25 +397,50 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
         if (stop > j.i0) {
             wait(O_FULL + t, 0u);
             smc_tc_fence_after();
-            const float norm = j.pieces > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-            T *dst = static_cast<T *>(u.out) + ((size_t)(j.r0 + tok) * u.heads + head) * HD;
+            const float norm = l == 0.0f ? 0.0f : 1.0f / l;
             float *part = work + ((size_t)blockIdx.x * PAIRS + m) * (HD + 4);
+            if (j.pieces > 1) {
 #pragma unroll 1
-            for (int k = 0; k < HD; k += 16) {
-                uint32_t o[16];
-                smc_tc_ld16(col_o + (uint32_t)k, o);
-                smc_tc_wait_ld();
-                if (real) {
+                for (int k = 0; k < HD; k += 16) {
+                    uint32_t o[16];
+                    smc_tc_ld16(col_o + (uint32_t)k, o);
+                    smc_tc_wait_ld();
+                    if (real) {
 #pragma unroll
-                    for (int e = 0; e < 16; e += 4) {
-                        const float v[4] = {__uint_as_float(o[e]) * norm, __uint_as_float(o[e + 1]) * norm, __uint_as_float(o[e + 2]) * norm, __uint_as_float(o[e + 3]) * norm};
-                        if (j.pieces > 1) smc_paged_store4(part + k + e, v);
-                        else smc_paged_store4(dst + k + e, v);
+                        for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4 *>(part + k + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    }
+                    __syncwarp();
+                }
+                if (real) part[HD] = R, part[HD + 1] = l;
+            } else {
+                // rows leave through the queries' shared memory, which no product reads any more: 16 bytes a lane, the lanes of a row side by side
+                constexpr int ROW = HD * (int)sizeof(T), CHUNKS = ROW / 16, N = 16 / (int)sizeof(T);
+                const uint32_t own = sbase + (uint32_t)t * S::Q_TILE + (uint32_t)(32 * (warp & 3)) * ROW;
+#pragma unroll
+                for (int k = 0; k < HD; k += 16) {
+                    uint32_t o[16];
+                    smc_tc_ld16(col_o + (uint32_t)k, o);
+                    smc_tc_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 16; e += N) {
+                        uint32_t v[4];
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            if constexpr (SPLIT) v[c] = __float_as_uint(__uint_as_float(o[e + c]) * norm);
+                            else v[c] = pack2(__uint_as_float(o[e + 2 * c]) * norm, __uint_as_float(o[e + 2 * c + 1]) * norm);
+                        }
+                        sts128(own + (uint32_t)(lane * ROW) + (uint32_t)((((k + e) / N) ^ (lane & 7)) * 16), v[0], v[1], v[2], v[3]);
                     }
                 }
                 __syncwarp();
+#pragma unroll 4
+                for (int i = lane; i < 32 * CHUNKS; i += 32) {
+                    const int r = i / CHUNKS, c = i % CHUNKS, at = t * TILE + 32 * (warp & 3) + r, pr = j.m0 + at, tk = pr / group;
+                    const uint4 v = smc_lds128(own + (uint32_t)(r * ROW + ((c ^ (r & 7)) * 16)));
+                    if (at < j.pairs)
+                        *reinterpret_cast<uint4 *>(static_cast<T *>(u.out) + ((size_t)(j.r0 + tk) * u.heads + j.h * group + pr - tk * group) * HD + c * N) = v;
+                }
             }
-            if (real && j.pieces > 1) part[HD] = R, part[HD + 1] = l;
         } else if (real && j.pieces > 1) {  // a piece behind the last key that this tile sees
             float *part = work + ((size_t)blockIdx.x * PAIRS + m) * (HD + 4);
             const float zero[4] = {};
