@@ -202,8 +202,8 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem + S::OFF_BAR + BARS * 8 + 4);
     auto bar = [&](int i) { return sbase + S::OFF_BAR + 8u * (uint32_t)i; };
-    auto wait = [&](int i, uint32_t parity) {  // by whole warps: one lane polls
-        if (lane == 0) smc_tc_wait(bar(i), parity & 1u, abort_flag, status);
+    auto wait = [&](int i, uint32_t parity) {  // by whole warps
+        smc_tc_wait(bar(i), parity & 1u, abort_flag, status);
         __syncwarp();
     };
     auto arrive = [&](int i) {
@@ -256,13 +256,22 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
             constexpr int N = 16 / (int)sizeof(T), LANES = HD / N, AT_ONCE = 32 / LANES;
             const int e = lane % LANES * N, sub = lane / LANES;
             float mine = 0.0f;  // the largest magnitude of this lane's own row
-#pragma unroll 4
-            for (int r = 0; r < 32; r += AT_ONCE) {
-                const int row = 32 * (warp & 3) + r + sub, at = t * TILE + row, pr = j.m0 + (at < j.pairs ? at : 0), tk = pr / group;
-                const T *src = static_cast<const T *>(u.q) + (long long)(j.r0 + tk) * u.q_stride + (size_t)(j.h * group + pr - tk * group) * HD + e;
+            constexpr int AHEAD = 8;
+            auto source = [&](int r) {
+                const int at = t * TILE + 32 * (warp & 3) + r + sub, pr = j.m0 + (at < j.pairs ? at : 0), tk = pr / group;
+                return reinterpret_cast<const uint4 *>(static_cast<const T *>(u.q) + (long long)(j.r0 + tk) * u.q_stride + (size_t)(j.h * group + pr - tk * group) * HD + e);
+            };
+#pragma unroll 1
+            for (int r0 = 0; r0 < 32; r0 += AHEAD * AT_ONCE) {
+              uint4 raw[AHEAD];
+#pragma unroll
+              for (int i = 0; i < AHEAD; ++i) raw[i] = *source(r0 + i * AT_ONCE);
+#pragma unroll
+              for (int i = 0; i < AHEAD; ++i) {
+                const int r = r0 + i * AT_ONCE, row = 32 * (warp & 3) + r + sub, at = t * TILE + row;
                 float v[N], most = 0.0f;
 #pragma unroll
-                for (int k = 0; k < N; k += 4) smc_paged_load4(src + k, *reinterpret_cast<float(*)[4]>(v + k));
+                for (int k = 0; k < N; ++k) v[k] = to_f(reinterpret_cast<const T *>(&raw[i])[k]);
 #pragma unroll
                 for (int k = 0; k < N; ++k) most = fmaxf(most, fabsf(v[k]));
 #pragma unroll
@@ -287,6 +296,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
                 } else {
                     sts128(dst, hi[0], hi[1], hi[2], hi[3]);
                 }
+              }
             }
             rowf = fabsf(u.scale) * 1.44269504088896341f * __uint_as_float((uint32_t)(127 - row_shift(mine)) << 23);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -299,12 +309,17 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
         for (int i = j.i0; i < stop; ++i) {
             const int it = i - j.i0, key0 = (j.kv0 + i) * KT;
             const uint32_t col_s = col_s0 + (uint32_t)((it & 1) * KT);
-            if (!there) wait(S_FULL + 2 * t + (it & 1), (uint32_t)(it >> 1));
+            if (!__all_sync(0xFFFFFFFFu, there)) wait(S_FULL + 2 * t + (it & 1), (uint32_t)(it >> 1));
             smc_tc_fence_after();
             uint32_t s[KT];
 #pragma unroll
             for (int k = 0; k < KT; k += 16) smc_tc_ld16(col_s + (uint32_t)k, *reinterpret_cast<uint32_t(*)[16]>(s + k));
+            float4 x[G];
             const float4 *sc = reinterpret_cast<const float4 *>(smem + S::OFF_SC) + (it % SC_SLOTS) * G;
+#pragma unroll
+            for (int k = 0; k < G; ++k) x[k] = sc[k];
+            // (asked here, the answer is there when this step is done)
+            there = i + 1 < stop && smc_mbar_test(bar(S_FULL + 2 * t + ((it + 1) & 1)), (uint32_t)((it + 1) >> 1) & 1u);
             smc_tc_wait_ld();
             const bool inner = key0 + KT <= lowest + 1 && (u.window <= 0 || key0 > highest - u.window);
             const int hi = inner ? KT : pos - key0, lo = !inner && u.window > 0 ? hi - u.window : -1;  // keys lo + 1 .. hi of the tile are seen
@@ -319,17 +334,11 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
                 }
             }
             // scales of 16 keys, for this row: a factor above 0, so that hidden keys stay -infinity; nothing of keys that are all hidden
-            auto scales = [&](int k) {
-                float4 x = sc[k];
-                x.x = fmaxf(x.x * rowf, 1e-37f);
-                if (16 * k > hi || 16 * k + 15 <= lo) x.y = -INFINITY, x.z = 0.0f;
-                return x;
-            };
-            float4 x[G];
 #pragma unroll
-            for (int k = 0; k < G; ++k) x[k] = scales(k);
-            // (asked here, the answer is there when this step is done)
-            there = i + 1 < stop && __all_sync(0xFFFFFFFFu, smc_mbar_test(bar(S_FULL + 2 * t + ((it + 1) & 1)), (uint32_t)((it + 1) >> 1) & 1u));
+            for (int k = 0; k < G; ++k) {
+                x[k].x = fmaxf(x[k].x * rowf, 1e-37f);
+                if (!inner && (16 * k > hi || 16 * k + 15 <= lo)) x[k].y = -INFINITY, x[k].z = 0.0f;
+            }
             float add;
 #pragma unroll 1
             for (bool again = true;;) {
