@@ -318,8 +318,6 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
             const float4 *sc = reinterpret_cast<const float4 *>(smem + S::OFF_SC) + (it % SC_SLOTS) * G;
 #pragma unroll
             for (int k = 0; k < G; ++k) x[k] = sc[k];
-            // (asked here, the answer is there when this step is done)
-            there = i + 1 < stop && smc_mbar_test(bar(S_FULL + 2 * t + ((it + 1) & 1)), (uint32_t)((it + 1) >> 1) & 1u);
             smc_tc_wait_ld();
             const bool inner = key0 + KT <= lowest + 1 && (u.window <= 0 || key0 > highest - u.window);
             const int hi = inner ? KT : pos - key0, lo = !inner && u.window > 0 ? hi - u.window : -1;  // keys lo + 1 .. hi of the tile are seen
@@ -399,6 +397,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
                 }
             }
             l += add;
+            there = i + 1 < stop && smc_mbar_test(bar(S_FULL + 2 * t + ((it + 1) & 1)), (uint32_t)((it + 1) >> 1) & 1u);  // (the answer comes under what follows)
             tmem_wait_st();
             smc_tc_fence_before();
             arrive(P_FULL + 2 * t + (it & 1));
