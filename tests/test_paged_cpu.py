@@ -24,7 +24,7 @@ def _cache(pages=4, kvh=2, page=16, dim=64):
     c = object.__new__(paged.PagedKVCache)
     c.torch, c.ctx, c.device = torch, _Ctx(), torch.device("cpu")
     c.pages, c.kv_heads, c.page, c.head_dim = pages, kvh, page, dim
-    c._types = {torch.float32: 0, torch.bfloat16: 30}
+    c._types, c._index, c._kv_ref = {torch.float32: 0, torch.bfloat16: 30}, -1, None  # (-1: the CPU)
     return c
 
 
