@@ -23,27 +23,35 @@ struct Update {
     int *status;
 };
 
-// four rotated neighbours of head `x` at dimension d; c, s: the position's rows of the tables
-template <typename T>
-__device__ __forceinline__ void rotated4(const T *x, int d, int rope_dim, bool neox, const float *c, const float *s, float (&y)[4])
+// Eight elements of a head, by unit 0 .. HD / 8 - 1: those of pairs (i, i + rope_dim / 2) in two fours where there is a rotation of that kind, neighbours
+// otherwise.  `second` is where the second four are.
+__device__ __forceinline__ void unit_place(int unit, int rope_dim, bool neox, int &first, int &second)
 {
-    smc_paged_load4(x + d, y);
-    if (!c || d >= rope_dim) return;
     const int half = rope_dim >> 1;
-    if (neox) {  // (i, i + half): half is a multiple of four
-        float p[4];
-        const bool low = d < half;
-        const int i = low ? d : d - half;
-        smc_paged_load4(x + (low ? d + half : d - half), p);
-        const float4 cc = *reinterpret_cast<const float4 *>(c + i), ss = *reinterpret_cast<const float4 *>(s + i);
+    if (neox && 4 * unit < half) first = 4 * unit, second = first + half;
+    else first = neox ? rope_dim + 2 * (4 * unit - half) : 8 * unit, second = first + 4;
+}
+// a[], b[]: the unit's elements, rotated by the position's rows of the tables; every product and sum is rounded
+__device__ __forceinline__ void unit_rotate(float (&a)[4], float (&b)[4], int first, int rope_dim, bool neox, const float *c, const float *s)
+{
+    if (first >= rope_dim) return;
+    if (neox) {
+        const float4 cc = *reinterpret_cast<const float4 *>(c + first), ss = *reinterpret_cast<const float4 *>(s + first);
         const float ca[4] = {cc.x, cc.y, cc.z, cc.w}, sa[4] = {ss.x, ss.y, ss.z, ss.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = low ? y[j] * ca[j] - p[j] * sa[j] : p[j] * sa[j] + y[j] * ca[j];
-    } else {  // (2 i, 2 i + 1)
-        const float2 cc = *reinterpret_cast<const float2 *>(c + (d >> 1)), ss = *reinterpret_cast<const float2 *>(s + (d >> 1));
-        const float a = y[0], b = y[1], e = y[2], f = y[3];
-        y[0] = a * cc.x - b * ss.x, y[1] = a * ss.x + b * cc.x;
-        y[2] = e * cc.y - f * ss.y, y[3] = e * ss.y + f * cc.y;
+        for (int j = 0; j < 4; ++j) {
+            const float x = a[j], y = b[j];
+            a[j] = x * ca[j] - y * sa[j], b[j] = x * sa[j] + y * ca[j];
+        }
+    } else {
+        const float4 cc = *reinterpret_cast<const float4 *>(c + (first >> 1)), ss = *reinterpret_cast<const float4 *>(s + (first >> 1));
+        const float ca[4] = {cc.x, cc.y, cc.z, cc.w}, sa[4] = {ss.x, ss.y, ss.z, ss.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float *p = j < 2 ? a + 2 * j : b + 2 * (j - 2);
+            const float x = p[0], y = p[1];
+            p[0] = x * ca[j] - y * sa[j], p[1] = x * sa[j] + y * ca[j];
+        }
     }
 }
 
@@ -55,32 +63,40 @@ __device__ __forceinline__ float block_scale(uint32_t amax)
     return __uint_as_float((uint32_t)(k + 127) << 23);
 }
 
-// Blocks of threads [0, items * kvh * 2): one page's new tokens of one head, keys or values.  The rest: rotated queries.
+// Blocks of threads [0, items * kvh * 2): one page's new tokens of one head, keys or values.  The rest: rotated queries, one row each.
 // Item i of the sequence with items [row_start / page + 2 s, ..): a sequence of n rows touches (n - 2) / page + 2 pages at most.
+// New values pass once through registers: their largest magnitude first, then, with the block's scale, their codes.  Keys: a thread takes units of
+// eight elements of a token; values, which lie with a dimension's tokens side by side: a dimension of up to PER_V tokens.
 template <typename T, int HD>
 __global__ void __launch_bounds__(UPDATE_THREADS) paged_update_kernel(const Update u)
 {
+    constexpr int UNITS = HD / 8, PER_K = 64 * UNITS / UPDATE_THREADS, GROUPS_V = UPDATE_THREADS / HD, PER_V = 64 / GROUPS_V;
     smc_grid_dep_sync();
     const smc_paged_view &c = u.c;
     const int page = 1 << c.shift, tid = threadIdx.x;
     const long long jobs = (long long)u.items * c.kvh * 2;
     if (blockIdx.x >= jobs) {
-        const long long at = (long long)(blockIdx.x - jobs) * UPDATE_THREADS + tid;
-        const int per_row = u.heads * (HD / 4);
-        const int r = (int)(at / per_row), e = (int)(at - (long long)r * per_row) * 4, d = e % HD;
-        const int s = r < c.rows ? smc_paged_row_sequence(c, r) : -1;
-        bool in = s >= 0;
-        float y[4];
-        if (in) {
-            const smc_paged_seq sq = smc_paged_sequence(c, s);
-            const int pos = sq.len - sq.n + r - sq.r0;
-            in = pos >= 0 && pos < u.table_rows;
-            if (!in && u.cosT) *u.status = SMC_STATUS_PAGED;
-            const size_t row = (size_t)pos * (u.rope_dim >> 1);
-            if (in) rotated4(static_cast<const T *>(u.q) + (long long)r * u.q_stride + (e - d), d, u.rope_dim, u.neox, u.cosT ? u.cosT + row : nullptr, u.sinT + row, y);
+        const int r = (int)(blockIdx.x - jobs), s = smc_paged_row_sequence(c, r);
+        if (s < 0) return;
+        const smc_paged_seq sq = smc_paged_sequence(c, s);
+        const int pos = sq.len - sq.n + r - sq.r0;
+        if (pos < 0 || pos >= u.table_rows) {
+            if (u.cosT && tid == 0) *u.status = SMC_STATUS_PAGED;
+            return;
         }
-        __syncwarp();  // in place: the two threads of a pair, both of one warp, have read it before either writes
-        if (in) smc_paged_store4(static_cast<T *>(u.q_out) + (long long)r * u.heads * HD + e, y);
+        const float *cs = u.cosT + (size_t)pos * (u.rope_dim >> 1), *sn = u.sinT + (size_t)pos * (u.rope_dim >> 1);
+        const T *src = static_cast<const T *>(u.q) + (long long)r * u.q_stride;
+        T *dst = static_cast<T *>(u.q_out) + (long long)r * u.heads * HD;
+#pragma unroll 2
+        for (int i = tid; i < u.heads * UNITS; i += UPDATE_THREADS) {  // (in place: a unit is read and written by one thread)
+            const int h = i / UNITS;
+            int first, second;
+            unit_place(i % UNITS, u.rope_dim, u.neox, first, second);
+            float a[4], b[4];
+            smc_paged_load4(src + h * HD + first, a), smc_paged_load4(src + h * HD + second, b);
+            unit_rotate(a, b, first, u.rope_dim, u.neox, cs, sn);
+            smc_paged_store4(dst + h * HD + first, a), smc_paged_store4(dst + h * HD + second, b);
+        }
         return;
     }
     const int item = (int)(blockIdx.x / (2 * c.kvh)), rest = (int)(blockIdx.x - (unsigned)item * 2 * c.kvh), h = rest >> 1;
@@ -109,28 +125,46 @@ __global__ void __launch_bounds__(UPDATE_THREADS) paged_update_kernel(const Upda
         return;
     }
     const int lo = max(p0 - start, 0), hi = min(sq.len - start, page);  // tokens [lo, hi) of the page are new
-    const T *src = static_cast<const T *>(values ? u.v : u.k) + (long long)(sq.r0 + start - p0) * (values ? u.v_stride : u.k_stride) + (size_t)h * HD;
     const long long stride = values ? u.v_stride : u.k_stride;
-    const size_t block = ((size_t)id * c.kvh + h) * ((size_t)HD << c.shift);
-    uint8_t *dst = (values ? c.v : c.k) + block;
+    const T *src = static_cast<const T *>(values ? u.v : u.k) + (long long)(sq.r0 + start - p0) * stride + (size_t)h * HD;  // of token 0
+    uint8_t *dst = (values ? c.v : c.k) + ((size_t)id * c.kvh + h) * ((size_t)HD << c.shift);
     float *scale = c.scales + ((size_t)id * c.kvh + h) * 2 + values;
-    const bool rotate = !values && u.cosT;
-    auto token4 = [&](int t, int d, float (&y)[4]) {
-        const size_t row = (size_t)(start + t) * (u.rope_dim >> 1);
-        rotated4(src + t * stride, d, u.rope_dim, u.neox, rotate ? u.cosT + row : nullptr, u.sinT + row, y);
-    };
-    constexpr int V = HD / 4;
+    const float old = lo > 0 ? *scale : 0.0f;
+
+    // ---- the new values and their largest magnitude
+    static_assert(PER_K * 8 == PER_V, "");
+    float x[PER_V];
+    const int d = tid % HD, t0 = tid / HD * (page / GROUPS_V), t1 = t0 + page / GROUPS_V;  // values: tokens [t0, t1) of dimension d
     uint32_t amax = 0;
-    for (int i = lo * V + tid; i < hi * V; i += UPDATE_THREADS) {
-        float y[4];
-        token4(i / V, i % V * 4, y);
+    if (values) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) amax = max(amax, __float_as_uint(y[j]) & 0x7FFFFFFFu);  // (as bits an undefined value is the largest)
+        for (int i = 0; i < PER_V; ++i) {
+            const int t = t0 + i;
+            x[i] = t < t1 && t >= lo && t < hi ? to_f(src[t * stride + d]) : 0.0f;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < PER_K; ++i) {
+            const int at = tid + i * UPDATE_THREADS, t = lo + at / UNITS;
+            int first, second;
+            unit_place(at % UNITS, u.rope_dim, u.neox, first, second);
+            float a[4] = {}, b[4] = {};
+            if (t < hi) {
+                smc_paged_load4(src + t * stride + first, a), smc_paged_load4(src + t * stride + second, b);
+                if (u.cosT) {
+                    const size_t row = (size_t)(start + t) * (u.rope_dim >> 1);
+                    unit_rotate(a, b, first, u.rope_dim, u.neox, u.cosT + row, u.sinT + row);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[8 * i + j] = a[j], x[8 * i + 4 + j] = b[j];
+        }
     }
+#pragma unroll
+    for (int i = 0; i < PER_V; ++i) amax = max(amax, __float_as_uint(x[i]) & 0x7FFFFFFFu);  // (as bits an undefined value is the largest)
     __shared__ uint32_t part[UPDATE_THREADS / 32];
     amax = __reduce_max_sync(0xFFFFFFFFu, amax);
     if ((tid & 31) == 0) part[tid >> 5] = amax;
-    const float old = lo > 0 ? *scale : 0.0f;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < UPDATE_THREADS / 32; ++i) amax = max(amax, part[i]);
@@ -138,69 +172,111 @@ __global__ void __launch_bounds__(UPDATE_THREADS) paged_update_kernel(const Upda
     const float now = old != old || need != need ? __uint_as_float(0x7FC00000u) : fmaxf(old, need);
     const float inv = now == now ? 1.0f / now : 0.0f;
     if (tid == 0 && !(now == old)) *scale = now;
-    if (lo > 0 && now > old) {  // the tokens that are there, under the new scale
+
+    // ---- tokens that are there, under the new scale
+    if (lo > 0 && now > old) {
         const float ratio = old * inv;
+        auto again = [&](uint32_t w) {
+            float f[4];
+            smc_e4m3x4_float(w, f);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[j] *= ratio;
+            return smc_float_e4m3x4(f);
+        };
         if (values) {
-            for (int i = tid; i < HD * lo; i += UPDATE_THREADS) {
-                uint8_t *p = dst + ((size_t)(i / lo) << c.shift) + i % lo;
-                float f[4];
-                smc_e4m3x4_float(*p, f);
-                f[0] *= ratio;
-                *p = (uint8_t)smc_float_e4m3x4(f);
+            for (int t = t0; t < min(t1, lo); t += 4) {
+                uint32_t *p = reinterpret_cast<uint32_t *>(dst + ((size_t)d << c.shift) + t);
+                const uint32_t was = *p, keep = t + 4 <= lo ? 0u : ~0u << (8 * (lo - t));  // bytes behind lo stay as they are
+                *p = (again(was) & ~keep) | (was & keep);
             }
         } else {
-            for (int i = tid; i < V * lo; i += UPDATE_THREADS) {
-                uint32_t *p = reinterpret_cast<uint32_t *>(dst) + i;
-                float f[4];
-                smc_e4m3x4_float(*p, f);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) f[j] *= ratio;
-                *p = smc_float_e4m3x4(f);
-            }
+            for (int i = tid; i < HD / 4 * lo; i += UPDATE_THREADS) reinterpret_cast<uint32_t *>(dst)[i] = again(reinterpret_cast<uint32_t *>(dst)[i]);
         }
     }
-    for (int i = lo * V + tid; i < hi * V; i += UPDATE_THREADS) {
-        const int t = i / V, d = i % V * 4;
-        float y[4];
-        token4(t, d, y);
+    // ---- codes of the new ones
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = now == now ? y[j] * inv : 0.0f;
-        const uint32_t w = smc_float_e4m3x4(y);
-        if (!values) *reinterpret_cast<uint32_t *>(dst + (size_t)t * HD + d) = w;
-        else
+    for (int i = 0; i < PER_V; ++i) x[i] = now == now ? x[i] * inv : 0.0f;
+    if (values) {
+        uint8_t *row = dst + ((size_t)d << c.shift) + t0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) dst[((size_t)(d + j) << c.shift) + t] = (uint8_t)(w >> (8 * j));
+        for (int i = 0; i < PER_V; i += 4) {
+            const int t = t0 + i;
+            if (t >= t1 || t + 4 <= lo || t >= hi) continue;
+            const uint32_t w = smc_float_e4m3x4(*reinterpret_cast<const float(*)[4]>(x + i));
+            if (t >= lo && t + 4 <= hi) *reinterpret_cast<uint32_t *>(row + i) = w;
+            else
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (t + j >= lo && t + j < hi) row[i + j] = (uint8_t)(w >> (8 * j));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < PER_K; ++i) {
+            const int at = tid + i * UPDATE_THREADS, t = lo + at / UNITS;
+            if (t >= hi) continue;
+            int first, second;
+            unit_place(at % UNITS, u.rope_dim, u.neox, first, second);
+            *reinterpret_cast<uint32_t *>(dst + (size_t)t * HD + first) = smc_float_e4m3x4(*reinterpret_cast<const float(*)[4]>(x + 8 * i));
+            *reinterpret_cast<uint32_t *>(dst + (size_t)t * HD + second) = smc_float_e4m3x4(*reinterpret_cast<const float(*)[4]>(x + 8 * i + 4));
+        }
     }
 }
 
-// One block of threads = one page and head.  K: four neighbours of a token a thread; V: sixteen tokens of a dimension.
+// One block of threads = one page and head.  K: eight neighbours of a token a thread; V: sixteen tokens of two dimensions.  All codes are on their way before the
+// first is written.
 template <typename T, int HD>
 __global__ void __launch_bounds__(128) paged_read_kernel(const smc_paged_view c, const int *pages, int n, T *k, T *v, int *status)
 {
+    constexpr int PER_K = 64 * HD / 8 / 128, PER_V = 4 * (HD / 2) / 128;
+    static_assert(PER_K >= 1 && PER_V >= 1, "");
     smc_grid_dep_sync();
-    const int i = blockIdx.x / c.kvh, h = blockIdx.x % c.kvh, id = pages[i], page = 1 << c.shift;
+    const int i = blockIdx.x / c.kvh, h = blockIdx.x % c.kvh, id = pages[i], page = 1 << c.shift, tid = threadIdx.x;
     const bool there = id >= 0 && id < c.pages;
-    if (!there && threadIdx.x == 0) *status = SMC_STATUS_PAGED;
+    if (!there && tid == 0) *status = SMC_STATUS_PAGED;
     const size_t block = there ? (size_t)id * c.kvh + h : 0, stride = (size_t)c.kvh * HD, at = ((size_t)i << c.shift) * stride + (size_t)h * HD;
-    const float sk = there ? c.scales[2 * block] : 0.0f, sv = there ? c.scales[2 * block + 1] : 0.0f;
+    const float2 scale = there ? *reinterpret_cast<const float2 *>(c.scales + 2 * block) : make_float2(0.0f, 0.0f);
     const uint8_t *pk = c.k + block * ((size_t)HD << c.shift), *pv = c.v + block * ((size_t)HD << c.shift);
-    for (int j = threadIdx.x; j < (HD / 4) << c.shift; j += 128) {
-        float f[4] = {};
-        if (there) smc_e4m3x4_float(reinterpret_cast<const uint32_t *>(pk)[j], f);
+    uint2 rk[PER_K];
+    uint4 rv[PER_V][2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] *= sk;
-        smc_paged_store4(k + at + (size_t)(j / (HD / 4)) * stride + j % (HD / 4) * 4, f);
+    for (int e = 0; e < PER_K; ++e) {
+        const int j = tid + 128 * e;
+        rk[e] = there && j < (HD / 8) << c.shift ? *reinterpret_cast<const uint2 *>(pk + 8 * j) : make_uint2(0, 0);
     }
-    for (int j = threadIdx.x; j < HD * (page / 16); j += 128) {
-        const int d = j % HD, t0 = j / HD * 16;
-        const uint4 raw = there ? *reinterpret_cast<const uint4 *>(pv + ((size_t)d << c.shift) + t0) : make_uint4(0, 0, 0, 0);
-        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float f[4];
-            smc_e4m3x4_float(w[e], f);
+    for (int e = 0; e < PER_V; ++e) {
+        const int j = tid + 128 * e, d = j % (HD / 2) * 2, t0 = j / (HD / 2) * 16;
+        const bool in = there && t0 < page;
+        rv[e][0] = in ? *reinterpret_cast<const uint4 *>(pv + ((size_t)d << c.shift) + t0) : make_uint4(0, 0, 0, 0);
+        rv[e][1] = in ? *reinterpret_cast<const uint4 *>(pv + ((size_t)(d + 1) << c.shift) + t0) : make_uint4(0, 0, 0, 0);
+    }
 #pragma unroll
-            for (int b = 0; b < 4; ++b) v[at + (size_t)(t0 + 4 * e + b) * stride + d] = from_f<T>(f[b] * sv);
+    for (int e = 0; e < PER_K; ++e) {
+        const int j = tid + 128 * e;
+        if (j >= (HD / 8) << c.shift) break;
+        float f[8];
+        smc_e4m3x4_float(rk[e].x, *reinterpret_cast<float(*)[4]>(f)), smc_e4m3x4_float(rk[e].y, *reinterpret_cast<float(*)[4]>(f + 4));
+#pragma unroll
+        for (int b = 0; b < 8; ++b) f[b] *= scale.x;
+        T *dst = k + at + (size_t)(j / (HD / 8)) * stride + j % (HD / 8) * 8;
+        if constexpr (sizeof(T) == 2) *reinterpret_cast<uint4 *>(dst) = make_uint4(pack2(f[0], f[1]), pack2(f[2], f[3]), pack2(f[4], f[5]), pack2(f[6], f[7]));
+        else smc_paged_store4(dst, *reinterpret_cast<float(*)[4]>(f)), smc_paged_store4(dst + 4, *reinterpret_cast<float(*)[4]>(f + 4));
+    }
+#pragma unroll
+    for (int e = 0; e < PER_V; ++e) {
+        const int j = tid + 128 * e, d = j % (HD / 2) * 2, t0 = j / (HD / 2) * 16;
+        if (t0 >= page) break;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            float a[4], b[4];
+            smc_e4m3x4_float(w == 0 ? rv[e][0].x : w == 1 ? rv[e][0].y : w == 2 ? rv[e][0].z : rv[e][0].w, a);
+            smc_e4m3x4_float(w == 0 ? rv[e][1].x : w == 1 ? rv[e][1].y : w == 2 ? rv[e][1].z : rv[e][1].w, b);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                T *dst = v + at + (size_t)(t0 + 4 * w + t) * stride + d;
+                if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t *>(dst) = pack2(a[t] * scale.y, b[t] * scale.y);
+                else *reinterpret_cast<float2 *>(dst) = make_float2(a[t] * scale.y, b[t] * scale.y);
+            }
         }
     }
 }
@@ -275,7 +351,7 @@ int smc_paged_update_dev(smc_ctx *ctx, const smc_paged_kv *kv, const smc_paged_s
     u.c = view(kv, seqs), u.k = d_k, u.v = d_v, u.q = d_q, u.q_out = d_q_out, u.k_stride = k_stride, u.v_stride = v_stride, u.q_stride = q_stride;
     u.heads = d_q ? heads : 0, u.rope_dim = d_cos ? rope_dim : 0, u.table_rows = d_cos ? table_rows : 0x7FFFFFFF, u.neox = neox, u.cosT = d_cos, u.sinT = d_sin, u.status = ctx->d_status;
     const long long items = seqs->row_start ? (seqs->rows >> u.c.shift) + 2LL * seqs->batch : seqs->batch;
-    const long long grid = items * kv->kv_heads * 2 + ((long long)seqs->rows * u.heads * (kv->head_dim / 4) + UPDATE_THREADS - 1) / UPDATE_THREADS;
+    const long long grid = items * kv->kv_heads * 2 + (d_q ? seqs->rows : 0);
     if (grid > 0x7FFFFFFF) return smc_fail(ctx, SMC_E_UNSUPPORTED, "paged_update: %lld rows and sequences in one call", (long long)seqs->rows + seqs->batch);
     u.items = (int)items;
     OnDevice on(ctx->device);

@@ -400,48 +400,75 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
     }
 }
 
-// One block of threads = one row and head, a thread a dimension: joins what the runs left of its segment, in their order.
+// One block of threads = one row and head: joins what the runs left of its segment.  Four dimensions a thread, the runs dealt to groups of threads, so that
+// all loads go out at once; each group adds its runs in their order, then the groups' sums are added in theirs.
+constexpr int JOIN_THREADS = 512;
 template <typename T, int HD>
-__global__ void __launch_bounds__(HD) paged_join_kernel(const smc_paged_view c, const smc_paged_query u, const float *__restrict__ work, int grid)
+__global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const smc_paged_view c, const smc_paged_query u, const float *__restrict__ work, int grid)
 {
+    constexpr int LANES = HD / 4, GROUPS = JOIN_THREADS / LANES;
     smc_grid_dep_sync();
-    const int group = u.heads / c.kvh, most = u.max_rows * group, m = blockIdx.x % most, h = blockIdx.x / most % c.kvh, s = blockIdx.x / most / c.kvh;
-    __shared__ int part[2][HD / 32];
+    const int group = u.heads / c.kvh, most = u.max_rows * group, m = blockIdx.x % most, h = blockIdx.x / most % c.kvh, s = blockIdx.x / most / c.kvh, tid = threadIdx.x;
+    __shared__ int part[2][JOIN_THREADS / 32];
+    __shared__ float tops[JOIN_THREADS / 32], sums[JOIN_THREADS / 32], factor[JOIN_THREADS];
+    __shared__ float4 outs[GROUPS][LANES];
     int before = 0, units = 0;
-    for (int i = threadIdx.x; i < c.batch; i += HD) {
+    for (int i = tid; i < c.batch; i += JOIN_THREADS) {
         const int n = c.kvh * span_of(c, u, i).tiles;
         units += n;
         if (i < s) before += n;
     }
     before = __reduce_add_sync(0xFFFFFFFFu, before), units = __reduce_add_sync(0xFFFFFFFFu, units);
-    if ((threadIdx.x & 31) == 0) part[0][threadIdx.x >> 5] = before, part[1][threadIdx.x >> 5] = units;
+    if ((tid & 31) == 0) part[0][tid >> 5] = before, part[1][tid >> 5] = units;
     __syncthreads();
     before = 0, units = 0;
 #pragma unroll
-    for (int i = 0; i < HD / 32; ++i) before += part[0][i], units += part[1][i];
+    for (int i = 0; i < JOIN_THREADS / 32; ++i) before += part[0][i], units += part[1][i];
     const Span p = span_of(c, u, s);
     if (m >= p.n * group) return;
-    const int runs = min(grid, units), begin = before + h * p.tiles, c0 = run_of(begin, runs, units), c1 = run_of(begin + p.tiles - 1, runs, units);
-    if (c0 == c1) return;  // whole in one run
-    float top = -INFINITY;
-    for (int i = c0; i <= c1; ++i) top = fmaxf(top, work[((size_t)i * 2 + (i == c0)) * most * (HD + 4) + (size_t)m * (HD + 4) + HD]);
-    const float ref = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, o = 0.0f;
+    const int runs = min(grid, units), begin = before + h * p.tiles, c0 = run_of(begin, runs, units), count = run_of(begin + p.tiles - 1, runs, units) - c0 + 1;
+    if (count == 1) return;  // whole in one run
+    auto row = [&](int i) { return work + ((size_t)(c0 + i) * 2 + (i == 0)) * most * (HD + 4) + (size_t)m * (HD + 4); };
+    // (one thread a run: a grid has no more than two an SM)
+    const float mine = tid < count ? row(tid)[HD] : -INFINITY, sum_mine = tid < count ? row(tid)[HD + 1] : 0.0f;
+    float top = mine;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    if ((tid & 31) == 0) tops[tid >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < JOIN_THREADS / 32; ++i) top = fmaxf(top, tops[i]);
+    const float f = ex2(mine - (top == -INFINITY ? 0.0f : top));
+    factor[tid] = f;
+    const float sum_warp = smc_group_sum<32>(tid < count ? sum_mine * f : 0.0f);
+    if ((tid & 31) == 0) sums[tid >> 5] = sum_warp;
+    __syncthreads();
+    const int g = tid / LANES, d = tid % LANES;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-    for (int i = c0; i <= c1; ++i) {
-        const float *row = work + ((size_t)i * 2 + (i == c0)) * most * (HD + 4) + (size_t)m * (HD + 4);
-        const float f = ex2(row[HD] - ref);
-        sum = fmaf(row[HD + 1], f, sum), o = fmaf(row[threadIdx.x], f, o);
+    for (int i = g; i < count; i += GROUPS) {
+        const float4 x = *reinterpret_cast<const float4 *>(row(i) + 4 * d);
+        const float w = factor[i];
+        o.x = fmaf(x.x, w, o.x), o.y = fmaf(x.y, w, o.y), o.z = fmaf(x.z, w, o.z), o.w = fmaf(x.w, w, o.w);
     }
-    const int tok = m / group;
-    static_cast<T *>(u.out)[((size_t)(p.r0 + tok) * u.heads + h * group + m - tok * group) * HD + threadIdx.x] = from_f<T>(sum == 0.0f ? 0.0f : o / sum);
+    outs[g][d] = o;
+    __syncthreads();
+    if (tid < HD) {
+        float sum = 0.0f, v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < JOIN_THREADS / 32; ++i) sum += sums[i];
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) v += reinterpret_cast<const float *>(&outs[i][0])[tid];
+        const int tok = m / group;
+        static_cast<T *>(u.out)[((size_t)(p.r0 + tok) * u.heads + h * group + m - tok * group) * HD + tid] = from_f<T>(sum == 0.0f ? 0.0f : v / sum);
+    }
 }
 
 // CTAs: two an SM, but four units (one a warp) each where there are that few
 int runs_for(const smc_ctx *ctx, int kvh, int batch, int max_len)
 {
     const long long bound = (long long)batch * kvh * std::max(1, (max_len + UNIT - 1) / UNIT);
-    return (int)std::min<long long>(2LL * ctx->sm_count, (bound + WARPS - 1) / WARPS);
+    return (int)std::min<long long>(std::min(2 * ctx->sm_count, JOIN_THREADS), (bound + WARPS - 1) / WARPS);
 }
 
 }  // namespace
@@ -459,7 +486,7 @@ int smc_launch_paged_decode(smc_ctx *ctx, const smc_paged_view &c, const smc_pag
     auto go = [&](auto main, auto join, int smem) {
         cudaFuncSetAttribute(main, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         smc_launch_dep(ctx->use_pdl, main, dim3(runs), dim3(THREADS), smem, s, c, u, work, ctx->d_status);
-        if (runs > 1) smc_launch_dep(ctx->use_pdl, join, dim3((unsigned)(c.batch * c.kvh * pairs)), dim3(u.hd), 0, s, c, u, work, runs);
+        if (runs > 1) smc_launch_dep(ctx->use_pdl, join, dim3((unsigned)(c.batch * c.kvh * pairs)), dim3(JOIN_THREADS), 0, s, c, u, work, runs);
     };
     if (u.bf16) {
         if (u.hd == 128) pairs <= 16 ? go(paged_decode_kernel<bf16, 128, 1>, paged_join_kernel<bf16, 128>, Ring<128>::SMEM) : go(paged_decode_kernel<bf16, 128, 2>, paged_join_kernel<bf16, 128>, Ring<128>::SMEM);
