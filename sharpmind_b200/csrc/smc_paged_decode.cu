@@ -5,12 +5,13 @@
 // warps take its units in turn.  What a CTA has of one sequence and head (a segment) is merged in shared memory at its end; a segment that a run's
 // border cuts leaves as (running maximum, sum, unnormalised output), and a second small kernel joins those.  The order of all sums is fixed by the lengths.
 //
-// A warp's unit: keys and values arrive by bulk copies in a ring of its own, K and V of 64 tokens a slot, two slots ahead.  Scores and outputs
-// are mma.sync m16n8k16 in fp16 with fp32 sums: an e4m3 code is exact in fp16, the queries are scaled by a power of two per row to 2^15 at most.  bfloat16
-// queries are exact so, 16 (row, head) pairs a tile; fp32 ones go in as hi + lo, 22 bits, in the tile's upper and lower eight rows, which costs
-// nothing where eight pairs are all there are.  Both products' contraction indices are permuted so that a thread reads 16 contiguous codes:
-// thread t of a quad owns dims [16 t, 16 t + 16) (and + 64) of the keys, and tokens [16 t, 16 t + 16) of scores, weights and values, which
-// lie in one page, so a unit's scales are two numbers a thread.
+// A warp's unit: keys and values arrive by bulk copies in a ring of its own, K or V of 64 tokens a slot, two slots ahead.  Scores and outputs
+// are mma.sync m16n8k16 in fp16 with fp32 sums, transposed: S^T = K Q^T and O^T = V^T P^T, so that the eight columns are the (row, query head) pairs, of which
+// there are few, and no tile is half empty.  An e4m3 code is exact in fp16; the queries are scaled by a power of two per row to 2^15 at most, which bfloat16
+// ones take exactly; fp32 queries and weights go in as hi + lo, 22 bits, into the same sums.
+// Both products' contraction indices are permuted so that a thread reads 16 contiguous codes: thread t of a quad takes dims [16 t, 16 t + 16) (and + 64) of
+// the keys, tokens [16 t, 16 t + 16) of the values.  The scores' row i of tile pair M is token 16 (i / 2) + 2 M + i % 2: a transposed eight by eight
+// block of weights (movmatrix) then is the second product's operand, and all tokens of a thread's scores lie in one page, so a unit's scales are two numbers.
 //   y_j = x_j log2(e) + log2(s_v);  w_j = 2^(y_j - M), M the running maximum of y less 14;  O = sum w_j code_j;  l = sum w_j / s_v;  out = O / l
 // The value scales ride in the exponent, so the weights stay within fp16 whatever the scales are: 2^14 at most, and 2^-38 of that still counts.
 #include "smc_async.cuh"
@@ -18,6 +19,7 @@
 
 namespace {
 
+constexpr int RUNS_MOST = 1024;
 constexpr int WARPS = 4, THREADS = 32 * WARPS, UNIT = 64, SLOTS = 3, CHUNKS = 256;
 constexpr float W_SHIFT = 14.0f;
 
@@ -45,6 +47,14 @@ __device__ __forceinline__ uint32_t rest_bits(float a, float b, uint32_t hi)
 {
     const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
     return half2_bits(a - h.x, b - h.y);
+}
+
+// an 8 x 8 matrix of halves, two of a row a thread, transposed
+__device__ __forceinline__ uint32_t transposed(uint32_t v)
+{
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
 }
 
 // tiles [t0, t0 + tiles) of 64 keys that rows of sequence s see; one tile, all masked, where there is no key, none where there is no row
@@ -82,11 +92,12 @@ __device__ __forceinline__ void advance(const smc_paged_view &c, const smc_paged
 // slot of a CTA's cut segment: 0 where it began before the run, 1 where it begins in it
 __device__ __forceinline__ float *partial(float *work, int cta, int which, int rows, int hd) { return work + ((size_t)cta * 2 + which) * rows * (hd + 4); }
 
-template <typename T, int HD, int MT>
-__global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_paged_view c, const smc_paged_query u, float *work, int *status)
+// NQ: (row, query head) pairs in eights
+template <typename T, int HD, int NQ>
+__global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_paged_view c, const smc_paged_query u, float *work, int aligned, int *status)
 {
-    constexpr bool SPLIT = sizeof(T) == 4;          // queries and weights as hi + lo
-    constexpr int ROWS = SPLIT ? 8 : 16, KS = HD / 16, CH = HD / 64, NT = HD / 8, OCT = SPLIT ? 1 : 2;
+    constexpr bool SPLIT = sizeof(T) == 4;  // queries and weights as hi + lo
+    constexpr int KS = HD / 16, CH = HD / 64, PL = SPLIT ? 2 : 1;
     using R = Ring<HD>;
     extern __shared__ __align__(128) uint8_t smem[];
     const uint32_t sbase = smc_smem_u32(smem);
@@ -130,9 +141,23 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
     }
     plan[2 * threadIdx.x] = before, plan[2 * threadIdx.x + 1] = before + mine[0];
     __syncthreads();
-    const int runs = min((int)gridDim.x, units);  // (no run between two others is empty)
-    if ((int)blockIdx.x >= runs) return;
-    const int first = run_first(blockIdx.x, runs, units), last = run_first(blockIdx.x + 1, runs, units);
+    int first, last;
+    if (aligned) {  // whole segments
+        auto unit_of = [&](long long segment) {
+            const int s1 = (int)(segment / c.kvh), g0 = s1 / per;
+            if (s1 >= c.batch) return units;
+            int before = plan[g0];
+            for (int s = g0 * per; s < s1; ++s) before += c.kvh * span_of(c, u, s).tiles;
+            return before + (int)(segment - (long long)s1 * c.kvh) * span_of(c, u, s1).tiles;
+        };
+        const long long segments = (long long)c.batch * c.kvh;
+        first = unit_of(blockIdx.x * segments / gridDim.x), last = unit_of((blockIdx.x + 1) * segments / gridDim.x);
+        if (first >= last) return;
+    } else {
+        const int runs = min((int)gridDim.x, units);  // (no run between two others is empty)
+        if ((int)blockIdx.x >= runs) return;
+        first = run_first(blockIdx.x, runs, units), last = run_first(blockIdx.x + 1, runs, units);
+    }
     Place at;
     {
         int lo = 0, hi = CHUNKS;  // the last group that starts at or before `first`
@@ -147,9 +172,9 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
     }
 
     // ---- what is on its way: half-stages K, V of this warp's units first + warp, + 4, ...
-    const int page = 1 << c.shift, pad = c.shift == 4 ? 32 : c.shift == 5 ? 64 : 0;
+    const int page = 1 << c.shift, pad = c.shift == 4 ? 32 : c.shift == 5 ? 64 : 0, g16 = g >> 1;
     struct Fetch {
-        int tile0, h, id, lo, hi;  // the unit's first key, its head, the page of this thread's 16 tokens (-1: nothing to bring); keys that count
+        int tile0, h, id, lo, hi;  // the unit's first key, its head, the page of tokens [16 g16, 16 g16 + 16) (-1: nothing to bring); keys that count
     };
     Place ahead = at;
     auto look = [&](int unit) {
@@ -159,7 +184,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
         const int rest = unit - ahead.base, h = rest / ahead.p.tiles;
         f.h = h, f.tile0 = (ahead.p.t0 + rest - h * ahead.p.tiles) * UNIT;
         f.lo = ahead.p.from, f.hi = ahead.p.len;
-        const int key = f.tile0 + 16 * t, p0 = key >> c.shift << c.shift;
+        const int key = f.tile0 + 16 * g16, p0 = key >> c.shift << c.shift;
         if (p0 + page > f.lo && p0 < f.hi) {  // (pages that left the window may have gone to another sequence)
             f.id = smc_paged_page(c, ahead.s, key >> c.shift);
             if (f.id < 0) *status = SMC_STATUS_PAGED;
@@ -169,7 +194,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
     auto scales_of = [&](const Fetch &f) {
         return f.id < 0 ? make_float2(0.0f, 1.0f) : *reinterpret_cast<const float2 *>(c.scales + 2 * ((size_t)f.id * c.kvh + f.h));
     };
-    const bool leader = g == 0 && ((16 * t) & (page - 1)) == 0;
+    const bool leader = (lane & 7) == 0 && ((16 * g16) & (page - 1)) == 0;
     auto request = [&](const Fetch &f, bool values, int slot) {
         const bool bring = leader && f.id >= 0;
         const unsigned who = __ballot_sync(0xFFFFFFFFu, bring);
@@ -177,7 +202,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
         __syncwarp();
         if (bring) {
             const size_t block = ((size_t)f.id * c.kvh + f.h) * ((size_t)HD << c.shift);
-            const uint32_t dst = ring + (uint32_t)(slot * R::SLOT + 16 * t * HD + (values ? ((16 * t) >> c.shift) * pad : 0));
+            const uint32_t dst = ring + (uint32_t)(slot * R::SLOT + 16 * g16 * HD + (values ? ((16 * g16) >> c.shift) * pad : 0));
             smc_bulk_g2s(dst, (values ? c.v : c.k) + block, (uint32_t)(page * HD), bars + 8 * slot);
         }
     };
@@ -195,143 +220,133 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
         const Span p = at.p;
         const int h = (seg - at.base) / p.tiles, begin = at.base + h * p.tiles, end = begin + p.tiles, stop = min(end, last);
         const int pairs = p.n * group;
-        uint32_t q[MT][KS][4];
-        float rowf[MT][OCT];
-        int pos[MT][OCT];
+        uint32_t q[NQ][PL][KS][2];
+        float rowf[NQ][2];  // of rows 2 t, 2 t + 1 of an eight, like all that follows
+        int pos[NQ][2];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nq = 0; nq < NQ; ++nq) {
+            const int m = min(8 * nq + g, pairs - 1), i = m / group;  // (rows behind the last repeat it and are not stored)
+            const T *src = static_cast<const T *>(u.q) + (long long)(p.r0 + i) * u.q_stride + (size_t)(h * group + m - i * group) * HD + 16 * t;
+            float x[4 * KS], most = 0.0f;
 #pragma unroll
-            for (int o = 0; o < OCT; ++o) {
-                const int m = min(mt * ROWS + 8 * o + g, pairs - 1), i = m / group;  // (rows behind the last repeat it and are not stored)
-                pos[mt][o] = p.len - p.n + i;
-                const T *src = static_cast<const T *>(u.q) + (long long)(p.r0 + i) * u.q_stride + (size_t)(h * group + m - i * group) * HD + 16 * t;
-                float x[4 * KS];
-                float most = 0.0f;
+            for (int e = 0; e < KS; ++e) {  // dims 64 (e / 4) + 16 t + 4 (e % 4)
+                smc_paged_load4(src + 64 * (e >> 2) + 4 * (e & 3), *reinterpret_cast<float(*)[4]>(x + 4 * e));
 #pragma unroll
-                for (int e = 0; e < KS; ++e) {  // dims 64 (e / 4) + 16 t + 4 (e % 4)
-                    float v[4];
-                    smc_paged_load4(src + 64 * (e >> 2) + 4 * (e & 3), v);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) x[4 * e + j] = v[j], most = fmaxf(most, fabsf(v[j]));
-                }
-                most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
-                most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
-                // the largest magnitude goes to [2^14, 2^15)
-                const int up = min(14 - ((int)(__float_as_uint(most) >> 23) - 127), 126);
-                const float fac = __uint_as_float((uint32_t)(up + 127) << 23);
-                rowf[mt][o] = u.scale * 1.44269504088896341f * __uint_as_float((uint32_t)(127 - up) << 23);
-#pragma unroll
-                for (int e = 0; e < KS; ++e) {
-                    const uint32_t a = half2_bits(x[4 * e] * fac, x[4 * e + 1] * fac), b = half2_bits(x[4 * e + 2] * fac, x[4 * e + 3] * fac);
-                    if constexpr (SPLIT) {
-                        q[mt][e][0] = a, q[mt][e][2] = b;
-                        q[mt][e][1] = rest_bits(x[4 * e] * fac, x[4 * e + 1] * fac, a), q[mt][e][3] = rest_bits(x[4 * e + 2] * fac, x[4 * e + 3] * fac, b);
-                    } else {
-                        q[mt][e][o] = a, q[mt][e][2 + o] = b;
-                    }
-                }
+                for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(x[4 * e + j]));
             }
-        float o[MT][NT][4] = {}, M[MT][OCT], l[MT][OCT];
+            most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
+            most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
+            // the largest magnitude goes to [2^14, 2^15)
+            const int up = min(14 - ((int)(__float_as_uint(most) >> 23) - 127), 126);
+            const float fac = __uint_as_float((uint32_t)(up + 127) << 23), back = u.scale * 1.44269504088896341f * __uint_as_float((uint32_t)(127 - up) << 23);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+            for (int e = 0; e < 2 * KS; ++e) {
+                const float a = x[2 * e] * fac, b = x[2 * e + 1] * fac;
+                q[nq][0][e >> 1][e & 1] = half2_bits(a, b);
+                if constexpr (SPLIT) q[nq][1][e >> 1][e & 1] = rest_bits(a, b, q[nq][0][e >> 1][e & 1]);
+            }
 #pragma unroll
-            for (int i = 0; i < OCT; ++i) M[mt][i] = -INFINITY, l[mt][i] = 0.0f;
+            for (int e = 0; e < 2; ++e) {
+                rowf[nq][e] = __shfl_sync(0xFFFFFFFFu, back, 4 * (2 * t + e));
+                pos[nq][e] = p.len - p.n + min(8 * nq + 2 * t + e, pairs - 1) / group;
+            }
+        }
+        float o[NQ][KS][4] = {}, M[NQ][2], l[NQ][2];
+#pragma unroll
+        for (int nq = 0; nq < NQ; ++nq) M[nq][0] = M[nq][1] = -INFINITY, l[nq][0] = l[nq][1] = 0.0f;
 
         for (; unit < stop; unit += WARPS) {
-            const int key0 = now.tile0 + 16 * t;  // this thread's tokens of scores and values
+            const int key0 = now.tile0 + 16 * g16 + (g & 1);  // this thread's tokens of the scores: key0 + 2 M
             later = look(unit + 2 * WARPS);
             sc_next = scales_of(next);
-            const bool here = now.id >= 0;
             // (a power of two's exponent; a scale that is none, left where no page is or undefined, stays what it is)
             const float bias = sc_now.y == sc_now.y ? (float)((int)(__float_as_uint(sc_now.y) >> 23) - 127) : sc_now.y, inv = 1.0f / sc_now.y;
             const bool inner = now.tile0 >= now.lo && now.tile0 + UNIT <= p.len - p.n + 1 && (u.window <= 0 || now.tile0 > p.len - 1 - u.window);
-            uint32_t w[MT][4][4];  // weights as A fragments
             landed(half);
+            float s[NQ][4][4] = {};
+            {
+                const uint32_t row = ring + (uint32_t)((half % SLOTS) * R::SLOT + (16 * g16 + (g & 1)) * HD + 16 * t);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                float s[8][4] = {};
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t row = ring + (uint32_t)((half % SLOTS) * R::SLOT + (16 * (g >> 1) + 2 * j + (g & 1)) * HD + 16 * t);
+                for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
                     for (int ch = 0; ch < CH; ++ch) {
-                        const uint4 raw = smc_lds128(row + 64 * ch);
-                        const uint32_t k4[4] = {raw.x, raw.y, raw.z, raw.w};
+                        const uint4 ra = smc_lds128(row + (uint32_t)(4 * mt * HD + 64 * ch)), rb = smc_lds128(row + (uint32_t)((4 * mt + 2) * HD + 64 * ch));
+                        const uint32_t wa[4] = {ra.x, ra.y, ra.z, ra.w}, wb[4] = {rb.x, rb.y, rb.z, rb.w};
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) mma_f16(s[j], q[mt][4 * ch + e], smc_e4m3x2_half2(k4[e] & 0xFFFFu), smc_e4m3x2_half2(k4[e] >> 16));
-                    }
-                }
-                float y[OCT][16];
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t a[4] = {smc_e4m3x2_half2(wa[e] & 0xFFFFu), smc_e4m3x2_half2(wb[e] & 0xFFFFu), smc_e4m3x2_half2(wa[e] >> 16), smc_e4m3x2_half2(wb[e] >> 16)};
 #pragma unroll
-                for (int i = 0; i < OCT; ++i) {
-                    const float f = rowf[mt][i] * sc_now.x;
+                            for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float acc = SPLIT ? s[j >> 1][j & 1] + s[j >> 1][2 + (j & 1)] : s[j >> 1][2 * i + (j & 1)];
-                        y[i][j] = fmaf(acc, f, bias);
-                    }
-                    if (!inner) {
-                        const int hi = min(pos[mt][i], p.len - 1), lo = u.window > 0 ? pos[mt][i] - u.window : -1;
-#pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (key0 + j > hi || key0 + j <= lo) y[i][j] = -INFINITY;
-                    }
-                    float top = y[i][0];
-#pragma unroll
-                    for (int j = 1; j < 16; ++j) top = fmaxf(top, y[i][j]);
-                    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-                    const float nm = fmaxf(M[mt][i], top - W_SHIFT), ref = nm == -INFINITY ? 0.0f : nm;
-                    const float corr = ex2(M[mt][i] - ref);  // (-inf: nothing yet, 0)
-                    M[mt][i] = nm;
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) sum += y[i][j] = ex2(y[i][j] - ref);
-                    // (a row that sees none of these tokens takes nothing of their scale, which may be undefined)
-                    l[mt][i] = fmaf(l[mt][i], corr, sum == 0.0f ? 0.0f : sum * inv);
-                    if (__any_sync(0xFFFFFFFFu, corr != 1.0f)) {
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            o[mt][n][2 * i] *= corr, o[mt][n][2 * i + 1] *= corr;
-                            if (SPLIT) o[mt][n][2] *= corr, o[mt][n][3] *= corr;
-                        }
-                    }
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int j = 4 * k + 2 * e;
-                        if constexpr (SPLIT) {
-                            w[mt][k][2 * e] = half2_bits(y[0][j], y[0][j + 1]);
-                            w[mt][k][2 * e + 1] = rest_bits(y[0][j], y[0][j + 1], w[mt][k][2 * e]);
-                        } else {
-                            w[mt][k][2 * e] = half2_bits(y[0][j], y[0][j + 1]);
-                            w[mt][k][2 * e + 1] = half2_bits(y[OCT - 1][j], y[OCT - 1][j + 1]);
+                                for (int pl = PL - 1; pl >= 0; --pl) mma_f16(s[nq][mt], a, q[nq][pl][4 * ch + e][0], q[nq][pl][4 * ch + e][1]);
                         }
                     }
             }
             __syncwarp();
             request(next, true, half % SLOTS);
             ++half;
+            uint32_t w[NQ][PL][8];  // weights as B fragments: block M of tokens
+#pragma unroll
+            for (int nq = 0; nq < NQ; ++nq) {
+                float corr[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float f = rowf[nq][r] * sc_now.x;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) s[nq][j >> 1][2 * (j & 1) + r] = fmaf(s[nq][j >> 1][2 * (j & 1) + r], f, bias);
+                    if (!inner) {
+                        const int hi = min(pos[nq][r], p.len - 1), lo = u.window > 0 ? pos[nq][r] - u.window : -1;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (key0 + 2 * j > hi || key0 + 2 * j <= lo) s[nq][j >> 1][2 * (j & 1) + r] = -INFINITY;
+                    }
+                    float top = s[nq][0][r];
+#pragma unroll
+                    for (int j = 1; j < 8; ++j) top = fmaxf(top, s[nq][j >> 1][2 * (j & 1) + r]);
+                    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
+                    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
+                    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
+                    const float nm = fmaxf(M[nq][r], top - W_SHIFT), ref = nm == -INFINITY ? 0.0f : nm;
+                    corr[r] = ex2(M[nq][r] - ref);  // (-inf: nothing yet, 0)
+                    M[nq][r] = nm;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) sum += s[nq][j >> 1][2 * (j & 1) + r] = ex2(s[nq][j >> 1][2 * (j & 1) + r] - ref);
+                    // (a row that sees none of these tokens takes nothing of their scale, which may be undefined)
+                    l[nq][r] = fmaf(l[nq][r], corr[r], sum == 0.0f ? 0.0f : sum * inv);
+                }
+                if (__any_sync(0xFFFFFFFFu, corr[0] != 1.0f || corr[1] != 1.0f)) {
+#pragma unroll
+                    for (int i = 0; i < KS; ++i) o[nq][i][0] *= corr[0], o[nq][i][1] *= corr[1], o[nq][i][2] *= corr[0], o[nq][i][3] *= corr[1];
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float a = s[nq][j >> 1][2 * (j & 1)], b = s[nq][j >> 1][2 * (j & 1) + 1];
+                    const uint32_t hi = half2_bits(a, b);
+                    w[nq][0][j] = transposed(hi);
+                    if constexpr (SPLIT) w[nq][1][j] = transposed(rest_bits(a, b, hi));
+                }
+            }
             landed(half);
             // values that do not count are zeros whatever their bytes are: the weights there are 0, and codes may be undefined
             uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
-            if (now.tile0 < now.lo || now.tile0 + UNIT > now.hi || !__all_sync(0xFFFFFFFFu, here)) {
+            if (now.tile0 < now.lo || now.tile0 + UNIT > now.hi) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    if (key0 + e < now.lo || key0 + e >= now.hi || !here) keep[e >> 2] &= ~(0xFFu << (8 * (e & 3)));
+                    if (now.tile0 + 16 * t + e < now.lo || now.tile0 + 16 * t + e >= now.hi) keep[e >> 2] &= ~(0xFFu << (8 * (e & 3)));
             }
             const uint32_t vbase = ring + (uint32_t)((half % SLOTS) * R::SLOT + ((16 * t) >> c.shift) * ((HD << c.shift) + pad) + ((16 * t) & (page - 1)));
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const uint4 raw = smc_lds128(vbase + (uint32_t)((8 * n + g) << c.shift));
-                const uint32_t v4[4] = {raw.x & keep[0], raw.y & keep[1], raw.z & keep[2], raw.w & keep[3]};
+            for (int i = 0; i < KS; ++i) {
+                const uint4 ra = smc_lds128(vbase + (uint32_t)((16 * i + g) << c.shift)), rb = smc_lds128(vbase + (uint32_t)((16 * i + 8 + g) << c.shift));
+                const uint32_t wa[4] = {ra.x & keep[0], ra.y & keep[1], ra.z & keep[2], ra.w & keep[3]}, wb[4] = {rb.x & keep[0], rb.y & keep[1], rb.z & keep[2], rb.w & keep[3]};
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const uint32_t b0 = smc_e4m3x2_half2(v4[k] & 0xFFFFu), b1 = smc_e4m3x2_half2(v4[k] >> 16);
+                    const uint32_t a[4] = {smc_e4m3x2_half2(wa[k] & 0xFFFFu), smc_e4m3x2_half2(wb[k] & 0xFFFFu), smc_e4m3x2_half2(wa[k] >> 16), smc_e4m3x2_half2(wb[k] >> 16)};
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) mma_f16(o[mt][n], w[mt][k], b0, b1);
+                    for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+                        for (int pl = PL - 1; pl >= 0; --pl) mma_f16(o[nq][i], a, w[nq][pl][2 * k], w[nq][pl][2 * k + 1]);
                 }
             }
             __syncwarp();
@@ -343,74 +358,75 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
         // ---- the segment's end: warps 1 .. leave what they have, warp 0 joins it, eight rows at a time
         const bool whole = begin >= first && end <= last;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nq = 0; nq < NQ; ++nq) {
+            if (8 * nq >= pairs) continue;  // (the same for all)
+            float sum[2];
 #pragma unroll
-            for (int i = 0; i < OCT; ++i) {
-                if (mt * ROWS + 8 * i >= pairs) continue;  // (the same for all)
-                float sum = l[mt][i];
-                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
-                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
-                __syncthreads();
-                if (warp > 0) {
-                    float *row = merge + ((warp - 1) * 8 + g) * R::MERGE_ROW;
-                    if (t == 0) row[HD] = M[mt][i], row[HD + 1] = sum;
+            for (int r = 0; r < 2; ++r) {
+                sum[r] = l[nq][r];
+                sum[r] += __shfl_xor_sync(0xFFFFFFFFu, sum[r], 4);
+                sum[r] += __shfl_xor_sync(0xFFFFFFFFu, sum[r], 8);
+                sum[r] += __shfl_xor_sync(0xFFFFFFFFu, sum[r], 16);
+            }
+            __syncthreads();
+            if (warp > 0) {
+                float *row = merge + ((warp - 1) * 8 + 2 * t) * R::MERGE_ROW;
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
-                        *reinterpret_cast<float2 *>(row + 8 * n + 2 * t) =
-                            SPLIT ? make_float2(o[mt][n][0] + o[mt][n][2], o[mt][n][1] + o[mt][n][3]) : make_float2(o[mt][n][2 * i], o[mt][n][2 * i + 1]);
+                for (int r = 0; r < 2; ++r) {
+                    if (g == 0) row[r * R::MERGE_ROW + HD] = M[nq][r], row[r * R::MERGE_ROW + HD + 1] = sum[r];
+#pragma unroll
+                    for (int i = 0; i < KS; ++i) row[r * R::MERGE_ROW + 16 * i + g] = o[nq][i][r], row[r * R::MERGE_ROW + 16 * i + 8 + g] = o[nq][i][2 + r];
                 }
-                __syncthreads();
-                if (warp == 0) {
-                    float top = M[mt][i];
+            }
+            __syncthreads();
+            if (warp == 0) {
 #pragma unroll
-                    for (int v = 0; v < WARPS - 1; ++v) top = fmaxf(top, merge[(v * 8 + g) * R::MERGE_ROW + HD]);
+                for (int r = 0; r < 2; ++r) {
+                    const float *rows = merge + (2 * t + r) * R::MERGE_ROW;
+                    float top = M[nq][r], fac[WARPS];
+#pragma unroll
+                    for (int v = 0; v < WARPS - 1; ++v) top = fmaxf(top, rows[v * 8 * R::MERGE_ROW + HD]);
                     const float ref = top == -INFINITY ? 0.0f : top;
-                    float fac[WARPS];
-                    fac[0] = ex2(M[mt][i] - ref);
-                    sum *= fac[0];
+                    fac[0] = ex2(M[nq][r] - ref);
+                    float all = sum[r] * fac[0];
 #pragma unroll
                     for (int v = 0; v < WARPS - 1; ++v) {
-                        const float *row = merge + (v * 8 + g) * R::MERGE_ROW;
-                        fac[v + 1] = ex2(row[HD] - ref);
-                        sum = fmaf(row[HD + 1], fac[v + 1], sum);
+                        fac[v + 1] = ex2(rows[v * 8 * R::MERGE_ROW + HD] - ref);
+                        all = fmaf(rows[v * 8 * R::MERGE_ROW + HD + 1], fac[v + 1], all);
                     }
-                    const int m = mt * ROWS + 8 * i + g, tok = m / group;
-                    const float norm = whole ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
+                    const int m = 8 * nq + 2 * t + r, tok = m / group;
+                    const float norm = whole ? (all == 0.0f ? 0.0f : 1.0f / all) : 1.0f;
                     float *part = partial(work, blockIdx.x, begin < first ? 0 : 1, u.max_rows * group, HD) + (size_t)m * (HD + 4);
                     T *dst = static_cast<T *>(u.out) + ((size_t)(p.r0 + tok) * u.heads + h * group + m - tok * group) * HD;
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        float a = (SPLIT ? o[mt][n][0] + o[mt][n][2] : o[mt][n][2 * i]) * fac[0], b = (SPLIT ? o[mt][n][1] + o[mt][n][3] : o[mt][n][2 * i + 1]) * fac[0];
+                    for (int i = 0; i < 2 * KS; ++i) {
+                        const int d = 8 * i + g;
+                        float a = o[nq][i >> 1][2 * (i & 1) + r] * fac[0];
 #pragma unroll
-                        for (int v = 0; v < WARPS - 1; ++v) {
-                            const float2 x = *reinterpret_cast<const float2 *>(merge + (v * 8 + g) * R::MERGE_ROW + 8 * n + 2 * t);
-                            a = fmaf(x.x, fac[v + 1], a), b = fmaf(x.y, fac[v + 1], b);
-                        }
-                        a *= norm, b *= norm;
+                        for (int v = 0; v < WARPS - 1; ++v) a = fmaf(rows[v * 8 * R::MERGE_ROW + d], fac[v + 1], a);
                         if (m < pairs) {
-                            if (!whole) *reinterpret_cast<float2 *>(part + 8 * n + 2 * t) = make_float2(a, b);
-                            else if constexpr (SPLIT) *reinterpret_cast<float2 *>(dst + 8 * n + 2 * t) = make_float2(a, b);
-                            else *reinterpret_cast<uint32_t *>(dst + 8 * n + 2 * t) = pack2(a, b);
+                            if (whole) dst[d] = from_f<T>(a * norm);
+                            else part[d] = a;
                         }
                     }
-                    if (!whole && m < pairs && t == 0) part[HD] = top, part[HD + 1] = sum;
+                    if (!whole && m < pairs && g == 0) part[HD] = top, part[HD + 1] = all;
                 }
             }
+        }
         seg = stop;
     }
 }
 
 // One block of threads = one row and head: joins what the runs left of its segment.  Four dimensions a thread, the runs dealt to groups of threads, so that
 // all loads go out at once; each group adds its runs in their order, then the groups' sums are added in theirs.
-constexpr int JOIN_THREADS = 512;
-template <typename T, int HD>
+template <typename T, int HD, int JOIN_THREADS>
 __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const smc_paged_view c, const smc_paged_query u, const float *__restrict__ work, int grid)
 {
     constexpr int LANES = HD / 4, GROUPS = JOIN_THREADS / LANES;
     smc_grid_dep_sync();
     const int group = u.heads / c.kvh, most = u.max_rows * group, m = blockIdx.x % most, h = blockIdx.x / most % c.kvh, s = blockIdx.x / most / c.kvh, tid = threadIdx.x;
     __shared__ int part[2][JOIN_THREADS / 32];
-    __shared__ float tops[JOIN_THREADS / 32], sums[JOIN_THREADS / 32], factor[JOIN_THREADS];
+    __shared__ float tops[JOIN_THREADS / 32], sums[JOIN_THREADS / 32], factor[RUNS_MOST];
     __shared__ float4 outs[GROUPS][LANES];
     int before = 0, units = 0;
     for (int i = tid; i < c.batch; i += JOIN_THREADS) {
@@ -429,18 +445,23 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const smc_page
     const int runs = min(grid, units), begin = before + h * p.tiles, c0 = run_of(begin, runs, units), count = run_of(begin + p.tiles - 1, runs, units) - c0 + 1;
     if (count == 1) return;  // whole in one run
     auto row = [&](int i) { return work + ((size_t)(c0 + i) * 2 + (i == 0)) * most * (HD + 4) + (size_t)m * (HD + 4); };
-    // (one thread a run: a grid has no more than two an SM)
-    const float mine = tid < count ? row(tid)[HD] : -INFINITY, sum_mine = tid < count ? row(tid)[HD + 1] : 0.0f;
-    float top = mine;
+    float top = -INFINITY, sum_mine = 0.0f;
+    for (int i = tid; i < count; i += JOIN_THREADS) {
+        factor[i] = row(i)[HD];
+        top = fmaxf(top, factor[i]);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
     if ((tid & 31) == 0) tops[tid >> 5] = top;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < JOIN_THREADS / 32; ++i) top = fmaxf(top, tops[i]);
-    const float f = ex2(mine - (top == -INFINITY ? 0.0f : top));
-    factor[tid] = f;
-    const float sum_warp = smc_group_sum<32>(tid < count ? sum_mine * f : 0.0f);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    for (int i = tid; i < count; i += JOIN_THREADS) {
+        factor[i] = ex2(factor[i] - ref);
+        sum_mine = fmaf(row(i)[HD + 1], factor[i], sum_mine);
+    }
+    const float sum_warp = smc_group_sum<32>(sum_mine);
     if ((tid & 31) == 0) sums[tid >> 5] = sum_warp;
     __syncthreads();
     const int g = tid / LANES, d = tid % LANES;
@@ -464,37 +485,47 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const smc_page
     }
 }
 
-// CTAs: two an SM, but four units (one a warp) each where there are that few
+template <int N> struct Dim {
+    static constexpr int v = N;
+};
+
+// Up to 8 tiles a segment, two a warp, its CTA goes through it alone and nothing is left to join (16 tiles alone: 18 us from cold caches, spread and joined 9 + 6); else
+// the units are spread evenly, over two CTAs an SM, but four units (one a warp) to each where there are that few.
+constexpr int ALONE = 8;
+int tiles_of(int max_len) { return std::max(1, (max_len + UNIT - 1) / UNIT); }
+bool alone(int max_len) { return tiles_of(max_len) <= ALONE; }
 int runs_for(const smc_ctx *ctx, int kvh, int batch, int max_len)
 {
-    const long long bound = (long long)batch * kvh * std::max(1, (max_len + UNIT - 1) / UNIT);
-    return (int)std::min<long long>(std::min(2 * ctx->sm_count, JOIN_THREADS), (bound + WARPS - 1) / WARPS);
+    const long long segments = (long long)batch * kvh, most = std::min(2 * ctx->sm_count, RUNS_MOST);
+    return (int)std::min(most, alone(max_len) ? segments : (segments * tiles_of(max_len) + WARPS - 1) / WARPS);
 }
 
 }  // namespace
 
-bool smc_paged_decode_takes(int bf16, int group, int max_rows) { return (long long)max_rows * group <= (bf16 ? 32 : 16); }
+bool smc_paged_decode_takes(int group, int max_rows) { return (long long)max_rows * group <= 16; }
 
 size_t smc_paged_decode_work(const smc_ctx *ctx, int kvh, int batch, int heads, int hd, int max_rows, int max_len)
 {
-    return (size_t)runs_for(ctx, kvh, batch, max_len) * 2 * max_rows * (heads / kvh) * (hd + 4) * sizeof(float);
+    return alone(max_len) ? 0 : (size_t)runs_for(ctx, kvh, batch, max_len) * 2 * max_rows * (heads / kvh) * (hd + 4) * sizeof(float);
 }
 
 int smc_launch_paged_decode(smc_ctx *ctx, const smc_paged_view &c, const smc_paged_query &u, float *work, cudaStream_t s)
 {
     const int pairs = u.max_rows * (u.heads / c.kvh), runs = runs_for(ctx, c.kvh, c.batch, u.max_len);
-    auto go = [&](auto main, auto join, int smem) {
-        cudaFuncSetAttribute(main, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        smc_launch_dep(ctx->use_pdl, main, dim3(runs), dim3(THREADS), smem, s, c, u, work, ctx->d_status);
-        if (runs > 1) smc_launch_dep(ctx->use_pdl, join, dim3((unsigned)(c.batch * c.kvh * pairs)), dim3(JOIN_THREADS), 0, s, c, u, work, runs);
+    const bool whole = alone(u.max_len), many = (long long)c.batch * c.kvh * pairs >= 1024;  // (many rows to join have few runs each)
+    auto pick = [&](auto type, auto hd) {
+        using T = decltype(type);
+        constexpr int HD = decltype(hd)::v;
+        auto main = pairs <= 8 ? paged_decode_kernel<T, HD, 1> : paged_decode_kernel<T, HD, 2>;
+        cudaFuncSetAttribute(main, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<HD>::SMEM);
+        smc_launch_dep(ctx->use_pdl, main, dim3(runs), dim3(THREADS), Ring<HD>::SMEM, s, c, u, work, whole ? 1 : 0, ctx->d_status);
+        if (whole || runs == 1) return;
+        const dim3 grid((unsigned)(c.batch * c.kvh * pairs));
+        if (many) smc_launch_dep(ctx->use_pdl, paged_join_kernel<T, HD, 128>, grid, dim3(128), 0, s, c, u, work, runs);
+        else smc_launch_dep(ctx->use_pdl, paged_join_kernel<T, HD, 512>, grid, dim3(512), 0, s, c, u, work, runs);
     };
-    if (u.bf16) {
-        if (u.hd == 128) pairs <= 16 ? go(paged_decode_kernel<bf16, 128, 1>, paged_join_kernel<bf16, 128>, Ring<128>::SMEM) : go(paged_decode_kernel<bf16, 128, 2>, paged_join_kernel<bf16, 128>, Ring<128>::SMEM);
-        else pairs <= 16 ? go(paged_decode_kernel<bf16, 64, 1>, paged_join_kernel<bf16, 64>, Ring<64>::SMEM) : go(paged_decode_kernel<bf16, 64, 2>, paged_join_kernel<bf16, 64>, Ring<64>::SMEM);
-    } else {
-        if (u.hd == 128) pairs <= 8 ? go(paged_decode_kernel<float, 128, 1>, paged_join_kernel<float, 128>, Ring<128>::SMEM) : go(paged_decode_kernel<float, 128, 2>, paged_join_kernel<float, 128>, Ring<128>::SMEM);
-        else pairs <= 8 ? go(paged_decode_kernel<float, 64, 1>, paged_join_kernel<float, 64>, Ring<64>::SMEM) : go(paged_decode_kernel<float, 64, 2>, paged_join_kernel<float, 64>, Ring<64>::SMEM);
-    }
+    if (u.bf16) u.hd == 128 ? pick(bf16(), Dim<128>()) : pick(bf16(), Dim<64>());
+    else u.hd == 128 ? pick(float(), Dim<128>()) : pick(float(), Dim<64>());
     SMC_LAUNCH_CHECK(ctx);
     return SMC_OK;
 }
