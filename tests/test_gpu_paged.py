@@ -302,6 +302,26 @@ def test_prompts_back_to_back(cuda, dtype, heads, dim):
     assert cuda.device_status() == 0
 
 
+@pytest.mark.parametrize("dtype,heads,kvh,dim", [(F32, 8, 8, 64), (BF16, 32, 8, 128), (BF16, 16, 8, 64)])
+def test_batches_whose_work_is_asked_for(cuda, dtype, heads, kvh, dim):
+    """Enough keys for short runs beside the equal ones, lengths far apart, replayed: the same bits each time, whoever took which run."""
+    lens = [20000, 3, 0, 9000, 700, 15000, 64, 5000, 1, 30000]
+    p = Pair(cuda, lens, kvh=kvh, dim=dim, page=64, tag="asked")
+    p.plain.k[:] = torch.randint(0, 112, p.plain.k.shape, dtype=torch.uint8, generator=gen("codes")) | (torch.randint(0, 2, p.plain.k.shape, dtype=torch.uint8, generator=gen("signs")) << 7)
+    p.plain.v[:] = p.plain.k.transpose(2, 3).flip(2)
+    p.plain.scales[:] = torch.exp2(torch.randint(-9, -5, p.plain.scales.shape, generator=gen("scales")).float())
+    p.upload()
+    q = randn((len(lens), heads, dim), "asked", heads).to(dtype)
+    first = p.cache.attention(q.cuda(), p.dtable, ints(lens), dim ** -0.5)
+    near(first, q, p, lens, [1] * len(lens), dim ** -0.5)
+    for _ in range(20):
+        assert torch.equal(first, p.cache.attention(q.cuda(), p.dtable, ints(lens), dim ** -0.5))
+    # shorter and longer than the call says
+    for long in (4000, 500000):
+        near(p.cache.attention(q.cuda(), p.dtable, ints(lens), dim ** -0.5, max_len=long), q, p, lens, [1] * len(lens), dim ** -0.5)
+    assert cuda.device_status() == 0
+
+
 # ---- where and when it runs
 @pytest.mark.parametrize("rows", [1, 3, 140])
 def test_captured_calls_serve_what_the_arrays_hold(cuda, rows):
