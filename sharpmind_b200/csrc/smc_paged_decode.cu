@@ -1,11 +1,9 @@
 // Attention of a few rows of every sequence over the paged cache (a decode step, drafts): the whole cache passes once through registers, so HBM is
 // the bound, and the work has to be even over the device whatever the sequences' lengths are.
 //
-// Units of 64 keys of one sequence and KV head, in the order (sequence, head, tile); the grid's CTAs take runs of them, a CTA's four
-// warps take its units in turn.  What a run has of one sequence and head (a segment) is merged in shared memory at its end; a segment that a run's
-// border cuts leaves as (running maximum, sum, unnormalised output), and a second small kernel joins those.  The runs, and with them the order of all sums,
-// are fixed by the lengths.  SMs get very different shares of the bandwidth (with equal runs the first CTA was done after 71 us, the last after 116), so large work
-// gives each CTA 60 % of an equal share and leaves the rest in short runs to whoever asks next.
+// Units of 64 keys of one sequence and KV head, in the order (sequence, head, tile); the grid's CTAs take equal runs of them, a CTA's four
+// warps take its units in turn.  What a CTA has of one sequence and head (a segment) is merged in shared memory at its end; a segment that a run's
+// border cuts leaves as (running maximum, sum, unnormalised output), and a second small kernel joins those.  The order of all sums is fixed by the lengths.
 //
 // A warp's unit: keys and values arrive by bulk copies in a ring of its own, K or V of 64 tokens a slot, two slots ahead.  Scores and outputs
 // are mma.sync m16n8k16 in fp16 with fp32 sums, transposed: S^T = K Q^T and O^T = V^T P^T, so that the eight columns are the (row, query head) pairs, of which
@@ -21,17 +19,17 @@
 
 namespace {
 
-constexpr int RUNS_MOST = 320 + 900 + 2;  // CTAs, short runs
+constexpr int RUNS_MOST = 1024;
 constexpr int WARPS = 4, THREADS = 32 * WARPS, UNIT = 64, SLOTS = 3, CHUNKS = 256;
 constexpr float W_SHIFT = 14.0f;
 
 template <int HD>
 struct Ring {
     static constexpr int SLOT = UNIT * HD + 128;               // values of 16- and 32-token pages lie 32 and 64 bytes further apart: no bank conflicts
-    static constexpr int OFF_MERGE = WARPS * SLOTS * SLOT;      // [warps 1 ..][8 rows][HD + 4] floats
-    static constexpr int MERGE_ROW = HD + 4;                    // O, then maximum and sum
-    static constexpr int OFF_BAR = OFF_MERGE + (WARPS - 1) * 8 * MERGE_ROW * 4, OFF_PLAN = OFF_BAR + WARPS * SLOTS * 8;
-    static constexpr int OFF_TOLD = OFF_PLAN + (CHUNKS + WARPS) * 4, SMEM = OFF_TOLD + 16;
+    static constexpr int OFF_MERGE = WARPS * SLOTS * SLOT;      // [warp][8 rows] of half of O, maximum and sum
+    static constexpr int MERGE_ROW = HD / 2 + 4;
+    static constexpr int OFF_BAR = OFF_MERGE + WARPS * 8 * MERGE_ROW * 4, OFF_PLAN = OFF_BAR + WARPS * SLOTS * 8;
+    static constexpr int SMEM = OFF_PLAN + (CHUNKS + WARPS) * 4 + 16;
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
@@ -74,28 +72,9 @@ __device__ __forceinline__ Span span_of(const smc_paged_view &c, const smc_paged
     p.tiles = p.n == 0 ? 0 : max(1, (sq.len + UNIT - 1) / UNIT - p.t0);
     return p;
 }
-// The runs of `units` units: `grid` equal ones, or (most > 0) 60 % in as many equal ones and the rest in up to `most` of 16 units or more.
-struct Runs {
-    int grid, units, most, each, tail, count;
-    __device__ __forceinline__ Runs(int grid_, int units_, int most_) : grid(min(grid_, units_)), units(units_), most(most_)
-    {
-        each = (int)((long long)units * 3 / 5 / max(grid, 1));
-        const int rest = units - each * grid;
-        if (each < 4 * WARPS) most = 0;
-        tail = most > 0 ? max(4 * WARPS, (rest + most - 1) / most) : 0;
-        count = most > 0 ? grid + (rest + tail - 1) / tail : grid;
-    }
-    __device__ __forceinline__ int first(int i) const
-    {
-        if (most == 0) return (int)((long long)i * units / grid);
-        return i <= grid ? i * each : min(units, each * grid + (i - grid) * tail);
-    }
-    __device__ __forceinline__ int of(int unit) const
-    {
-        if (most == 0) return (int)(((long long)(unit + 1) * grid - 1) / units);
-        return unit < each * grid ? unit / each : grid + (unit - each * grid) / tail;
-    }
-};
+// run of units of CTA i of n: [first, first of the next)
+__device__ __forceinline__ int run_first(int i, int n, int units) { return (int)((long long)i * units / n); }
+__device__ __forceinline__ int run_of(int unit, int n, int units) { return (int)(((long long)(unit + 1) * n - 1) / units); }
 
 // Where a warp is among the units: sequence s has [base, base + kvh * tiles)
 struct Place {
@@ -110,12 +89,12 @@ __device__ __forceinline__ void advance(const smc_paged_view &c, const smc_paged
     }
 }
 
-// slot of a run's cut segment: 0 where it began before the run, 1 where it begins in it
-__device__ __forceinline__ float *partial(float *work, int run, int which, int rows, int hd) { return work + ((size_t)run * 2 + which) * rows * (hd + 4); }
+// slot of a CTA's cut segment: 0 where it began before the run, 1 where it begins in it
+__device__ __forceinline__ float *partial(float *work, int cta, int which, int rows, int hd) { return work + ((size_t)cta * 2 + which) * rows * (hd + 4); }
 
 // NQ: (row, query head) pairs in eights
 template <typename T, int HD, int NQ>
-__global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_paged_view c, const smc_paged_query u, float *work, int aligned, int most, int *ticket, int *status)
+__global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_paged_view c, const smc_paged_query u, float *work, int aligned, int *status)
 {
     constexpr bool SPLIT = sizeof(T) == 4;  // queries and weights as hi + lo
     constexpr int KS = HD / 16, CH = HD / 64, PL = SPLIT ? 2 : 1;
@@ -129,7 +108,6 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
     int *plan = reinterpret_cast<int *>(smem + R::OFF_PLAN), *sums = plan + CHUNKS;
     if (lane == 0) {
         for (int i = 0; i < SLOTS; ++i) smc_mbar_init(bars + 8 * i, 1);
-        if (warp == 0) smc_mbar_init(sbase + (uint32_t)R::OFF_TOLD, 1);
         smc_fence_barrier_init();
     }
     smc_grid_dep_sync();
@@ -163,21 +141,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
     }
     plan[2 * threadIdx.x] = before, plan[2 * threadIdx.x + 1] = before + mine[0];
     __syncthreads();
-    const Runs runs((int)gridDim.x, units, aligned ? 0 : most);
-    auto place = [&](int unit) {
-        Place w;
-        int lo = 0, hi = CHUNKS;  // the last group that starts at or before the unit
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (plan[mid] <= unit) lo = mid;
-            else hi = mid;
-        }
-        // (groups behind the last sequence start at `units`)
-        w.s = min(lo * per, c.batch - 1), w.base = plan[lo], w.p = span_of(c, u, w.s);
-        advance(c, u, w, unit);
-        return w;
-    };
-    int run = blockIdx.x, first, last;
+    int first, last;
     if (aligned) {  // whole segments
         auto unit_of = [&](long long segment) {
             const int s1 = (int)(segment / c.kvh), g0 = s1 / per;
@@ -190,23 +154,22 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
         first = unit_of(blockIdx.x * segments / gridDim.x), last = unit_of((blockIdx.x + 1) * segments / gridDim.x);
         if (first >= last) return;
     } else {
-        if (run >= runs.grid) return;
-        first = runs.first(run), last = runs.first(run + 1);  // (no run between two others is empty)
+        const int runs = min((int)gridDim.x, units);  // (no run between two others is empty)
+        if ((int)blockIdx.x >= runs) return;
+        first = run_first(blockIdx.x, runs, units), last = run_first(blockIdx.x + 1, runs, units);
     }
-    const bool more = runs.most > 0;  // runs to be asked for
-    // The next run's number is asked for when a run begins; whoever needs it, ahead of the run's end, waits for it.
-    const uint32_t told = sbase + (uint32_t)R::OFF_TOLD;
-    volatile int *next_run = reinterpret_cast<volatile int *>(smem + R::OFF_TOLD + 8);  // [run's parity]
-    int asked = 0;  // runs this CTA has begun
-    auto ask = [&]() {
-        if (more && threadIdx.x == 0) {
-            next_run[asked & 1] = runs.grid + atomicAdd(ticket, 1);
-            smc_mbar_arrive(told);
+    Place at;
+    {
+        int lo = 0, hi = CHUNKS;  // the last group that starts at or before `first`
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (plan[mid] <= first) lo = mid;
+            else hi = mid;
         }
-        ++asked;
-    };
-    ask();
-    Place at = place(first);
+        // (groups behind the last sequence start at `units`)
+        at.s = min(lo * per, c.batch - 1), at.base = plan[lo], at.p = span_of(c, u, at.s);
+        advance(c, u, at, first);
+    }
 
     // ---- what is on its way: half-stages K, V of this warp's units first + warp, + 4, ...
     const int page = 1 << c.shift, pad = c.shift == 4 ? 32 : c.shift == 5 ? 64 : 0, g16 = g >> 1;
@@ -214,22 +177,9 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
         int tile0, h, id, lo, hi;  // the unit's first key, its head, the page of tokens [16 g16, 16 g16 + 16) (-1: nothing to bring); keys that count
     };
     Place ahead = at;
-    int ahead_unit = first + warp, ahead_last = last, ahead_run = run, ahead_asked = 1;
-    auto look = [&]() {  // at this warp's next unit (a run has four for each warp, the last of all aside, so one look ahead of a run is enough)
+    auto look = [&](int unit) {
         Fetch f{0, 0, -1, 0, 0};
-        if (ahead_unit >= ahead_last) {
-            if (!more || ahead_run >= runs.count - 1 || ahead_asked > asked) return f;
-            if (!smc_mbar_wait(told, (uint32_t)(ahead_asked - 1) & 1u)) *status = 4;
-            ahead_run = next_run[(ahead_asked - 1) & 1];
-            ++ahead_asked;
-            if (ahead_run >= runs.count) return f;
-            const int begin = runs.first(ahead_run);
-            ahead = place(begin);
-            ahead_unit = begin + warp, ahead_last = runs.first(ahead_run + 1);
-            if (ahead_unit >= ahead_last) return f;
-        }
-        const int unit = ahead_unit;
-        ahead_unit += WARPS;
+        if (unit >= last) return f;
         advance(c, u, ahead, unit);
         const int rest = unit - ahead.base, h = rest / ahead.p.tiles;
         f.h = h, f.tile0 = (ahead.p.t0 + rest - h * ahead.p.tiles) * UNIT;
@@ -260,20 +210,12 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
         if (!smc_mbar_wait(bars + 8 * (half % SLOTS), (uint32_t)(half / SLOTS) & 1u)) *status = 4;
     };
     int unit = first + warp, half = 0;
-    Fetch now = look(), next = look(), later;
+    Fetch now = look(unit), next = look(unit + WARPS), later;
     float2 sc_now = scales_of(now), sc_next;
     request(now, false, 0), request(now, true, 1), request(next, false, 2);
 
     // ---- segments
-    for (int seg = first;;) {
-        if (seg >= last) {  // the next run
-            if (!more || run >= runs.count - 1) break;
-            run = ahead_run;  // (this warp has looked two units behind its last one)
-            if (run >= runs.count) break;
-            first = runs.first(run), last = runs.first(run + 1), seg = first, unit = first + warp;
-            at = place(first);
-            ask();
-        }
+    for (int seg = first; seg < last;) {
         advance(c, u, at, seg);
         const Span p = at.p;
         const int h = (seg - at.base) / p.tiles, begin = at.base + h * p.tiles, end = begin + p.tiles, stop = min(end, last);
@@ -315,7 +257,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
 
         for (; unit < stop; unit += WARPS) {
             const int key0 = now.tile0 + 16 * g16 + (g & 1);  // this thread's tokens of the scores: key0 + 2 M
-            later = look();
+            later = look(unit + 2 * WARPS);
             sc_next = scales_of(next);
             // (a power of two's exponent; a scale that is none, left where no page is or undefined, stays what it is)
             const float bias = sc_now.y == sc_now.y ? (float)((int)(__float_as_uint(sc_now.y) >> 23) - 127) : sc_now.y, inv = 1.0f / sc_now.y;
@@ -413,7 +355,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
             now = next, next = later, sc_now = sc_next;
         }
 
-        // ---- the segment's end: warps 1 .. leave what they have, warp 0 joins it, eight rows at a time
+        // ---- the segment's end: the warps' sums, eight rows at a time
         const bool whole = begin >= first && end <= last;
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq) {
@@ -426,48 +368,46 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
                 sum[r] += __shfl_xor_sync(0xFFFFFFFFu, sum[r], 8);
                 sum[r] += __shfl_xor_sync(0xFFFFFFFFu, sum[r], 16);
             }
-            __syncthreads();
-            if (warp > 0) {
-                float *row = merge + ((warp - 1) * 8 + 2 * t) * R::MERGE_ROW;
+            // half of the dimensions at a time; warp w then adds rows 2 w, 2 w + 1 of all
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+                __syncthreads();
+                float *row = merge + (warp * 8 + 2 * t) * R::MERGE_ROW;
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    if (g == 0) row[r * R::MERGE_ROW + HD] = M[nq][r], row[r * R::MERGE_ROW + HD + 1] = sum[r];
+                    if (part == 0 && g == 0) row[r * R::MERGE_ROW + HD / 2] = M[nq][r], row[r * R::MERGE_ROW + HD / 2 + 1] = sum[r];
 #pragma unroll
-                    for (int i = 0; i < KS; ++i) row[r * R::MERGE_ROW + 16 * i + g] = o[nq][i][r], row[r * R::MERGE_ROW + 16 * i + 8 + g] = o[nq][i][2 + r];
+                    for (int i = 0; i < KS / 2; ++i)
+                        row[r * R::MERGE_ROW + 16 * i + g] = o[nq][part * (KS / 2) + i][r], row[r * R::MERGE_ROW + 16 * i + 8 + g] = o[nq][part * (KS / 2) + i][2 + r];
                 }
-            }
-            __syncthreads();
-            if (warp == 0) {
+                __syncthreads();
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const float *rows = merge + (2 * t + r) * R::MERGE_ROW;
-                    float top = M[nq][r], fac[WARPS];
+                    const float *rows = merge + (2 * warp + r) * R::MERGE_ROW;  // of warp v: + 8 v rows
+                    const int m = 8 * nq + 2 * warp + r, tok = m / group;
+                    if (m >= pairs) continue;
+                    float top = -INFINITY, fac[WARPS], all = 0.0f;
 #pragma unroll
-                    for (int v = 0; v < WARPS - 1; ++v) top = fmaxf(top, rows[v * 8 * R::MERGE_ROW + HD]);
+                    for (int v = 0; v < WARPS; ++v) top = fmaxf(top, rows[v * 8 * R::MERGE_ROW + HD / 2]);
                     const float ref = top == -INFINITY ? 0.0f : top;
-                    fac[0] = ex2(M[nq][r] - ref);
-                    float all = sum[r] * fac[0];
 #pragma unroll
-                    for (int v = 0; v < WARPS - 1; ++v) {
-                        fac[v + 1] = ex2(rows[v * 8 * R::MERGE_ROW + HD] - ref);
-                        all = fmaf(rows[v * 8 * R::MERGE_ROW + HD + 1], fac[v + 1], all);
+                    for (int v = 0; v < WARPS; ++v) {
+                        fac[v] = ex2(rows[v * 8 * R::MERGE_ROW + HD / 2] - ref);
+                        all = fmaf(rows[v * 8 * R::MERGE_ROW + HD / 2 + 1], fac[v], all);
                     }
-                    const int m = 8 * nq + 2 * t + r, tok = m / group;
                     const float norm = whole ? (all == 0.0f ? 0.0f : 1.0f / all) : 1.0f;
-                    float *part = partial(work, run, begin < first ? 0 : 1, u.max_rows * group, HD) + (size_t)m * (HD + 4);
+                    float *part_row = partial(work, blockIdx.x, begin < first ? 0 : 1, u.max_rows * group, HD) + (size_t)m * (HD + 4);
                     T *dst = static_cast<T *>(u.out) + ((size_t)(p.r0 + tok) * u.heads + h * group + m - tok * group) * HD;
 #pragma unroll
-                    for (int i = 0; i < 2 * KS; ++i) {
-                        const int d = 8 * i + g;
-                        float a = o[nq][i >> 1][2 * (i & 1) + r] * fac[0];
+                    for (int i = 0; i < HD / 64; ++i) {
+                        float a = 0.0f;
 #pragma unroll
-                        for (int v = 0; v < WARPS - 1; ++v) a = fmaf(rows[v * 8 * R::MERGE_ROW + d], fac[v + 1], a);
-                        if (m < pairs) {
-                            if (whole) dst[d] = from_f<T>(a * norm);
-                            else part[d] = a;
-                        }
+                        for (int v = 0; v < WARPS; ++v) a = fmaf(rows[v * 8 * R::MERGE_ROW + 32 * i + lane], fac[v], a);
+                        const int d = part * (HD / 2) + 32 * i + lane;
+                        if (whole) dst[d] = from_f<T>(a * norm);
+                        else part_row[d] = a;
                     }
-                    if (!whole && m < pairs && g == 0) part[HD] = top, part[HD + 1] = all;
+                    if (!whole && part == 0 && lane == 0) part_row[HD] = top, part_row[HD + 1] = all;
                 }
             }
         }
@@ -478,7 +418,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
 // One block of threads = one row and head: joins what the runs left of its segment.  Four dimensions a thread, the runs dealt to groups of threads, so that
 // all loads go out at once; each group adds its runs in their order, then the groups' sums are added in theirs.
 template <typename T, int HD, int JOIN_THREADS>
-__global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const smc_paged_view c, const smc_paged_query u, const float *__restrict__ work, int grid, int tails)
+__global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const smc_paged_view c, const smc_paged_query u, const float *__restrict__ work, int grid)
 {
     constexpr int LANES = HD / 4, GROUPS = JOIN_THREADS / LANES;
     smc_grid_dep_sync();
@@ -500,8 +440,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const smc_page
     for (int i = 0; i < JOIN_THREADS / 32; ++i) before += part[0][i], units += part[1][i];
     const Span p = span_of(c, u, s);
     if (m >= p.n * group) return;
-    const Runs runs(grid, units, tails);
-    const int begin = before + h * p.tiles, c0 = runs.of(begin), count = runs.of(begin + p.tiles - 1) - c0 + 1;
+    const int runs = min(grid, units), begin = before + h * p.tiles, c0 = run_of(begin, runs, units), count = run_of(begin + p.tiles - 1, runs, units) - c0 + 1;
     if (count == 1) return;  // whole in one run
     auto row = [&](int i) { return work + ((size_t)(c0 + i) * 2 + (i == 0)) * most * (HD + 4) + (size_t)m * (HD + 4); };
     float top = -INFINITY, sum_mine = 0.0f;
@@ -555,16 +494,8 @@ int tiles_of(int max_len) { return std::max(1, (max_len + UNIT - 1) / UNIT); }
 bool alone(int max_len) { return tiles_of(max_len) <= ALONE; }
 int runs_for(const smc_ctx *ctx, int kvh, int batch, int max_len)
 {
-    const long long segments = (long long)batch * kvh, most = std::min(2 * ctx->sm_count, 320);
+    const long long segments = (long long)batch * kvh, most = std::min(2 * ctx->sm_count, RUNS_MOST);
     return (int)std::min(most, alone(max_len) ? segments : (segments * tiles_of(max_len) + WARPS - 1) / WARPS);
-}
-
-// Short runs to be asked for: where a CTA has 32 units (half a megabyte of heads of 128) and more, which is worth the ticket's clearing
-int tails_for(const smc_ctx *ctx, int kvh, int batch, int max_len)
-{
-    const long long units = (long long)batch * kvh * tiles_of(max_len);
-    if (alone(max_len) || units < 32LL * runs_for(ctx, kvh, batch, max_len)) return 0;
-    return (int)std::min(900LL, units * 2 / 5 / (4 * WARPS) + 1);
 }
 
 }  // namespace
@@ -573,28 +504,23 @@ bool smc_paged_decode_takes(int group, int max_rows) { return (long long)max_row
 
 size_t smc_paged_decode_work(const smc_ctx *ctx, int kvh, int batch, int heads, int hd, int max_rows, int max_len)
 {
-    if (alone(max_len)) return 0;
-    return 16 + ((size_t)runs_for(ctx, kvh, batch, max_len) + tails_for(ctx, kvh, batch, max_len) + 1) * 2 * max_rows * (heads / kvh) * (hd + 4) * sizeof(float);
+    return alone(max_len) ? 0 : (size_t)runs_for(ctx, kvh, batch, max_len) * 2 * max_rows * (heads / kvh) * (hd + 4) * sizeof(float);
 }
 
 int smc_launch_paged_decode(smc_ctx *ctx, const smc_paged_view &c, const smc_paged_query &u, float *work, cudaStream_t s)
 {
     const int pairs = u.max_rows * (u.heads / c.kvh), runs = runs_for(ctx, c.kvh, c.batch, u.max_len);
-    const int tails = tails_for(ctx, c.kvh, c.batch, u.max_len);
-    int *ticket = reinterpret_cast<int *>(work);  // the work space's first 16 bytes
-    if (work) work += 4;
-    if (tails > 0) SMC_CUDA(ctx, cudaMemsetAsync(ticket, 0, sizeof(int), s));
     const bool whole = alone(u.max_len), many = (long long)c.batch * c.kvh * pairs >= 1024;  // (many rows to join have few runs each)
     auto pick = [&](auto type, auto hd) {
         using T = decltype(type);
         constexpr int HD = decltype(hd)::v;
         auto main = pairs <= 8 ? paged_decode_kernel<T, HD, 1> : paged_decode_kernel<T, HD, 2>;
         cudaFuncSetAttribute(main, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<HD>::SMEM);
-        smc_launch_dep(ctx->use_pdl, main, dim3(runs), dim3(THREADS), Ring<HD>::SMEM, s, c, u, work, whole ? 1 : 0, tails, ticket, ctx->d_status);
+        smc_launch_dep(ctx->use_pdl, main, dim3(runs), dim3(THREADS), Ring<HD>::SMEM, s, c, u, work, whole ? 1 : 0, ctx->d_status);
         if (whole || runs == 1) return;
         const dim3 grid((unsigned)(c.batch * c.kvh * pairs));
-        if (many) smc_launch_dep(ctx->use_pdl, paged_join_kernel<T, HD, 128>, grid, dim3(128), 0, s, c, u, work, runs, tails);
-        else smc_launch_dep(ctx->use_pdl, paged_join_kernel<T, HD, 512>, grid, dim3(512), 0, s, c, u, work, runs, tails);
+        if (many) smc_launch_dep(ctx->use_pdl, paged_join_kernel<T, HD, 128>, grid, dim3(128), 0, s, c, u, work, runs);
+        else smc_launch_dep(ctx->use_pdl, paged_join_kernel<T, HD, 512>, grid, dim3(512), 0, s, c, u, work, runs);
     };
     if (u.bf16) u.hd == 128 ? pick(bf16(), Dim<128>()) : pick(bf16(), Dim<64>());
     else u.hd == 128 ? pick(float(), Dim<128>()) : pick(float(), Dim<64>());
