@@ -16,7 +16,7 @@
 
 namespace {
 
-constexpr int PAIRS = 256, TILE = 128, KT = 64, G = KT / 16, SOFT_WARPS = 8, CONV_WARP = 8, MMA_WARP = 12, THREADS = 32 * (MMA_WARP + 2), SC_SLOTS = 8;
+constexpr int PAIRS = 256, TILE = 128, KT = 64, G = KT / 16, SOFT_WARPS = 8, CONV_WARP = 8, MMA_WARP = 12, THREADS = 32 * (MMA_WARP + 2), SC_SLOTS = 8, STEPS_LEAST = 4, SPLIT_SMS = 2;  // (a piece of a job has four steps at least, in fp32, whose queries are longer in coming, eight)
 constexpr float R_BELOW = 6.0f, SUM_MOST = 65000.0f;
 
 // A wait names a phase by its parity: no barrier passes a phase before its waiter has seen the one before.  (PV_DONE may for a softmax, which looks
@@ -25,7 +25,7 @@ enum { FULL = 0, EMPTY = 4, S_FULL = 8, P_FULL = 12 /* [tile][step parity] */, P
 
 template <int HD, bool SPLIT>
 struct Shape {
-    static constexpr int PLANES = SPLIT ? 2 : 1, STAGES = SPLIT ? 2 : 4;
+    static constexpr int PLANES = SPLIT ? 2 : 1, STAGES = 2;  // (each stage has its own copy of the MMAs: four were slower, the SM's instruction cache has enough to hold)
     static constexpr uint32_t SUB_Q = TILE * 128, Q_PLANE = HD / 64 * SUB_Q, Q_TILE = PLANES * Q_PLANE;
     static constexpr uint32_t HALF = KT * HD * 2, STAGE = 2 * HALF;  // fp16 keys of a step, values of the last step but one
     static constexpr uint32_t OFF_K = 2 * Q_TILE, OFF_SC = OFF_K + STAGES * STAGE, OFF_BAR = OFF_SC + SC_SLOTS * G * 16, SMEM = OFF_BAR + 256;
@@ -160,6 +160,19 @@ __device__ __forceinline__ void issue_mmas(uint32_t sbase, int mine, int n, uint
         });
 }
 
+// Row and head within the group of every step-th pair, divided once
+struct PairWalk {
+    int row, head, group, rows, heads;
+    __device__ __forceinline__ PairWalk(int pair, int group_, int step) : row(pair / group_), group(group_), rows(step / group_)
+    {
+        head = pair - row * group, heads = step - rows * group;
+    }
+    __device__ __forceinline__ void next()
+    {
+        row += rows, head += heads;
+        if (head >= group) head -= group, ++row;
+    }
+};
 // What a CTA does: pairs [m0, m0 + pairs) of sequence s and head h; key tiles [kv0, kv0 + n[t]) of tile t, of which this piece takes [i0, i1).
 struct Job {
     int s, h, m0, pairs, len, n_rows, r0, from, kv0, n0, n1, i0, i1, piece, pieces;
@@ -186,7 +199,7 @@ __device__ __forceinline__ bool job_of(const smc_paged_view &c, const smc_paged_
     j.from = u.window > 0 ? max(0, first - u.window + 1) : 0;
     j.kv0 = j.from / KT;
     j.n0 = max(1, (end0 + KT - 1) / KT - j.kv0), j.n1 = j.pairs > TILE ? max(j.n0, (end1 + KT - 1) / KT - j.kv0) : j.n0;
-    j.pieces = min(split, j.n1), j.piece = piece;
+    j.pieces = min(split, max(1, j.n1 / (u.bf16 ? STEPS_LEAST : 2 * STEPS_LEAST))), j.piece = piece;
     if (piece >= j.pieces) return false;
     j.i0 = (int)((long long)piece * j.n1 / j.pieces), j.i1 = (int)((long long)(piece + 1) * j.n1 / j.pieces);
     return true;
@@ -250,46 +263,67 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
         const int pair = j.m0 + (real ? m : 0), tok = pair / group;
         const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16), col_s0 = lanes + S::COL_S + (uint32_t)(2 * t * KT), col_o = lanes + S::COL_O + (uint32_t)(t * HD);
         const int pos = j.len - j.n_rows + tok;
+        // 16 bytes of the warp's own rows in its tile's queries
+        auto own = [&](int row, int chunk) {
+            const int block = chunk >> 3;
+            return sbase + (uint32_t)t * S::Q_TILE + (uint32_t)(block / (HD / 64)) * S::Q_PLANE + (uint32_t)(block % (HD / 64)) * S::SUB_Q + (uint32_t)(32 * (warp & 3) + row) * 128u +
+                   (uint32_t)(((chunk & 7) ^ (row & 7)) << 4);
+        };
         float rowf = 0.0f, R = -INFINITY, l = 0.0f;
         if (stop > j.i0) {
-            // the warp's 32 rows, 16 bytes a lane, the lanes of a row side by side
+            // the warp's 32 rows, 16 bytes a lane, the lanes of a row side by side; a short loop, four of a lane's loads ahead: code that is
+            // gone through once a CTA costs its fetch
             constexpr int N = 16 / (int)sizeof(T), LANES = HD / N, AT_ONCE = 32 / LANES;
             const int e = lane % LANES * N, sub = lane / LANES;
             float mine = 0.0f;  // the largest magnitude of this lane's own row
-            constexpr int AHEAD = 8;
-            auto source = [&](int r) {
-                const int at = t * TILE + 32 * (warp & 3) + r + sub, pr = j.m0 + (at < j.pairs ? at : 0), tk = pr / group;
-                return reinterpret_cast<const uint4 *>(static_cast<const T *>(u.q) + (long long)(j.r0 + tk) * u.q_stride + (size_t)(j.h * group + pr - tk * group) * HD + e);
+            constexpr int AHEAD = 4;
+            PairWalk from(j.m0 + t * TILE + 32 * (warp & 3) + sub, group, AT_ONCE);
+            const T *const q0 = static_cast<const T *>(u.q) + (long long)j.r0 * u.q_stride + (size_t)(j.h * group) * HD + e;
+            uint4 next[AHEAD];
+            auto fetch = [&](int r0) {
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) {
+                    const bool in = r0 < 32 && t * TILE + 32 * (warp & 3) + r0 + i * AT_ONCE + sub < j.pairs;
+                    next[i] = in ? *reinterpret_cast<const uint4 *>(q0 + (long long)from.row * u.q_stride + (size_t)from.head * HD) : make_uint4(0, 0, 0, 0);
+                    from.next();
+                }
             };
+            fetch(0);
 #pragma unroll 1
             for (int r0 = 0; r0 < 32; r0 += AHEAD * AT_ONCE) {
               uint4 raw[AHEAD];
 #pragma unroll
-              for (int i = 0; i < AHEAD; ++i) raw[i] = *source(r0 + i * AT_ONCE);
+              for (int i = 0; i < AHEAD; ++i) raw[i] = next[i];
+              fetch(r0 + AHEAD * AT_ONCE);
+              float tops[AHEAD];
 #pragma unroll
               for (int i = 0; i < AHEAD; ++i) {
-                const int r = r0 + i * AT_ONCE, row = 32 * (warp & 3) + r + sub, at = t * TILE + row;
-                float v[N], most = 0.0f;
+                tops[i] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < N; ++k) tops[i] = fmaxf(tops[i], fabsf(to_f(reinterpret_cast<const T *>(&raw[i])[k])));
+              }
+#pragma unroll
+              for (int o = LANES / 2; o > 0; o >>= 1)
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) tops[i] = fmaxf(tops[i], __shfl_xor_sync(0xFFFFFFFFu, tops[i], o));
+#pragma unroll
+              for (int i = 0; i < AHEAD; ++i) {
+                const int r = r0 + i * AT_ONCE, row = 32 * (warp & 3) + r + sub;
+                const float most = tops[i], theirs = __shfl_sync(0xFFFFFFFFu, most, (lane % AT_ONCE) * LANES);
+                if (lane / AT_ONCE * AT_ONCE == r) mine = theirs;
+                float v[N];
 #pragma unroll
                 for (int k = 0; k < N; ++k) v[k] = to_f(reinterpret_cast<const T *>(&raw[i])[k]);
-#pragma unroll
-                for (int k = 0; k < N; ++k) most = fmaxf(most, fabsf(v[k]));
-#pragma unroll
-                for (int o = LANES / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
-                const float theirs = __shfl_sync(0xFFFFFFFFu, most, (lane % AT_ONCE) * LANES);
-                if (lane / AT_ONCE * AT_ONCE == r) mine = theirs;
                 // the largest magnitude of the row goes to [2^14, 2^15); a negative scale turns the queries' sign
                 float fac = __uint_as_float((uint32_t)(row_shift(most) + 127) << 23);
                 if (u.scale < 0.0f) fac = -fac;
-                if (at >= j.pairs) fac = 0.0f;
                 uint32_t hi[N / 2], lo[N / 2];
 #pragma unroll
                 for (int k = 0; k < N / 2; ++k) {
                     hi[k] = half2_bits(v[2 * k] * fac, v[2 * k + 1] * fac);
                     if (SPLIT) lo[k] = rest_bits(v[2 * k] * fac, v[2 * k + 1] * fac, hi[k]);
                 }
-                const uint32_t dst = sbase + (uint32_t)t * S::Q_TILE + (uint32_t)(e >> 6) * S::SUB_Q + (uint32_t)(row >> 3) * 1024u + (uint32_t)(row & 7) * 128u +
-                                     (uint32_t)((((e >> 3) & 7) ^ (row & 7)) << 4);
+                const uint32_t dst = own(row & 31, e >> 3);
                 if constexpr (SPLIT) {
                     const uint32_t half = (uint32_t)(e & 4) * 2u;
                     smc_sts64(dst + half, make_uint2(hi[0], hi[1])), smc_sts64(dst + S::Q_PLANE + half, make_uint2(lo[0], lo[1]));
@@ -406,49 +440,49 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
             wait(O_FULL + t, 0u);
             smc_tc_fence_after();
             const float norm = l == 0.0f ? 0.0f : 1.0f / l;
-            float *part = work + ((size_t)blockIdx.x * PAIRS + m) * (HD + 4);
-            if (j.pieces > 1) {
+            // Rows leave through the queries' shared memory, which no product reads any more: a lane its own row first, then 16 bytes a lane with the lanes of a
+            // row side by side.  Results, or what a piece has of O, half a row (fp32: a row) at a time.
+            constexpr int N = 16 / (int)sizeof(T), AT_ONCE = S::PLANES * HD / 2;
+            const bool piece = j.pieces > 1;
+            float *part = work + ((size_t)blockIdx.x * PAIRS) * (HD + 4);
 #pragma unroll 1
-                for (int k = 0; k < HD; k += 16) {
-                    uint32_t o[16];
-                    smc_tc_ld16(col_o + (uint32_t)k, o);
-                    smc_tc_wait_ld();
-                    if (real) {
+            for (int k0 = 0; k0 < HD; k0 += AT_ONCE) {
+                uint32_t o[AT_ONCE];
 #pragma unroll
-                        for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4 *>(part + k + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                    }
-                    __syncwarp();
-                }
-                if (real) part[HD] = R, part[HD + 1] = l;
-            } else {
-                // rows leave through the queries' shared memory, which no product reads any more: 16 bytes a lane, the lanes of a row side by side
-                constexpr int ROW = HD * (int)sizeof(T), CHUNKS = ROW / 16, N = 16 / (int)sizeof(T);
-                const uint32_t own = sbase + (uint32_t)t * S::Q_TILE + (uint32_t)(32 * (warp & 3)) * ROW;
+                for (int k = 0; k < AT_ONCE; k += 16) smc_tc_ld16(col_o + (uint32_t)(k0 + k), *reinterpret_cast<uint32_t(*)[16]>(o + k));
+                smc_tc_wait_ld();
+                if (piece || SPLIT) {
+                    const float by = piece ? 1.0f : norm;
 #pragma unroll
-                for (int k = 0; k < HD; k += 16) {
-                    uint32_t o[16];
-                    smc_tc_ld16(col_o + (uint32_t)k, o);
-                    smc_tc_wait_ld();
+                    for (int e = 0; e < AT_ONCE; e += 4)
+                        sts128(own(lane, e / 4), __float_as_uint(__uint_as_float(o[e]) * by), __float_as_uint(__uint_as_float(o[e + 1]) * by),
+                               __float_as_uint(__uint_as_float(o[e + 2]) * by), __float_as_uint(__uint_as_float(o[e + 3]) * by));
+                } else {
 #pragma unroll
-                    for (int e = 0; e < 16; e += N) {
-                        uint32_t v[4];
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            if constexpr (SPLIT) v[c] = __float_as_uint(__uint_as_float(o[e + c]) * norm);
-                            else v[c] = pack2(__uint_as_float(o[e + 2 * c]) * norm, __uint_as_float(o[e + 2 * c + 1]) * norm);
-                        }
-                        sts128(own + (uint32_t)(lane * ROW) + (uint32_t)((((k + e) / N) ^ (lane & 7)) * 16), v[0], v[1], v[2], v[3]);
-                    }
+                    for (int e = 0; e < AT_ONCE; e += 8)
+                        sts128(own(lane, e / 8), pack2(__uint_as_float(o[e]) * norm, __uint_as_float(o[e + 1]) * norm), pack2(__uint_as_float(o[e + 2]) * norm, __uint_as_float(o[e + 3]) * norm),
+                               pack2(__uint_as_float(o[e + 4]) * norm, __uint_as_float(o[e + 5]) * norm), pack2(__uint_as_float(o[e + 6]) * norm, __uint_as_float(o[e + 7]) * norm));
                 }
                 __syncwarp();
-#pragma unroll 4
-                for (int i = lane; i < 32 * CHUNKS; i += 32) {
-                    const int r = i / CHUNKS, c = i % CHUNKS, at = t * TILE + 32 * (warp & 3) + r, pr = j.m0 + at, tk = pr / group;
-                    const uint4 v = smc_lds128(own + (uint32_t)(r * ROW + ((c ^ (r & 7)) * 16)));
-                    if (at < j.pairs)
-                        *reinterpret_cast<uint4 *>(static_cast<T *>(u.out) + ((size_t)(j.r0 + tk) * u.heads + j.h * group + pr - tk * group) * HD + c * N) = v;
+                if (piece) {
+                    constexpr int CHUNKS = AT_ONCE / 4;
+#pragma unroll 2
+                    for (int r = lane / CHUNKS, c = lane % CHUNKS; r < 32; r += 32 / CHUNKS) {
+                        const int at = t * TILE + 32 * (warp & 3) + r;
+                        if (at < j.pairs) *reinterpret_cast<uint4 *>(part + (size_t)at * (HD + 4) + k0 + 4 * c) = smc_lds128(own(r, c));
+                    }
+                } else {
+                    constexpr int CHUNKS = AT_ONCE / N;
+                    PairWalk to(j.m0 + t * TILE + 32 * (warp & 3) + lane / CHUNKS, group, 32 / CHUNKS);
+                    T *const out0 = static_cast<T *>(u.out) + ((size_t)j.r0 * u.heads + j.h * group) * HD + k0 + lane % CHUNKS * N;
+#pragma unroll 2
+                    for (int r = lane / CHUNKS; r < 32; r += 32 / CHUNKS, to.next())
+                        if (t * TILE + 32 * (warp & 3) + r < j.pairs)
+                            *reinterpret_cast<uint4 *>(out0 + ((size_t)to.row * u.heads + to.head) * HD) = smc_lds128(own(r, lane % CHUNKS));
                 }
+                __syncwarp();
             }
+            if (piece && real) part[(size_t)m * (HD + 4) + HD] = R, part[(size_t)m * (HD + 4) + HD + 1] = l;
         } else if (real && j.pieces > 1) {  // a piece behind the last key that this tile sees
             float *part = work + ((size_t)blockIdx.x * PAIRS + m) * (HD + 4);
             const float zero[4] = {};
@@ -553,30 +587,50 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
     }
 }
 
-// One warp = one pair of a job whose keys were split: joins the pieces in their order.
-template <typename T, int HD>
+// One warp = JOIN_WARP pairs of a job whose keys were split: joins the pieces in their order.
+template <typename T, int HD, int JOIN_WARP>
 __global__ void __launch_bounds__(256) paged_prompt_join_kernel(const smc_paged_view c, const smc_paged_query u, int items, int split, const float *__restrict__ work)
 {
     smc_grid_dep_sync();
-    constexpr int E = HD / 32;
-    const int lane = threadIdx.x & 31, b = blockIdx.x / (PAIRS / 8), m = blockIdx.x % (PAIRS / 8) * 8 + (threadIdx.x >> 5);
+    constexpr int E = HD / 32, JOIN_PAIRS = 8 * JOIN_WARP;
+    const int lane = threadIdx.x & 31, b = blockIdx.x / (PAIRS / JOIN_PAIRS), m0 = blockIdx.x % (PAIRS / JOIN_PAIRS) * JOIN_PAIRS + (threadIdx.x >> 5) * JOIN_WARP;
     Job j;
-    if (!job_of(c, u, items - 1 - b / c.kvh, b % c.kvh, 0, split, j, nullptr) || j.pieces == 1 || m >= j.pairs) return;
-    const float *row = work + ((size_t)b * split * PAIRS + m) * (HD + 4);
+    if (!job_of(c, u, items - 1 - b / c.kvh, b % c.kvh, 0, split, j, nullptr) || j.pieces == 1 || m0 >= j.pairs) return;
     const size_t step = (size_t)PAIRS * (HD + 4);
-    float top = -INFINITY, sum = 0.0f, o[E] = {};
-    for (int i = 0; i < j.pieces; ++i) top = fmaxf(top, row[i * step + HD]);
-    const float ref = top == -INFINITY ? 0.0f : top;
-    for (int i = 0; i < j.pieces; ++i) {
-        const float f = ex2(row[i * step + HD] - ref);
-        sum = fmaf(row[i * step + HD + 1], f, sum);
+    const int group = u.heads / c.kvh;
+    const float *row[JOIN_WARP];
+    float2 end[JOIN_WARP];  // a lane a piece: R and l
+    float o[JOIN_WARP][E] = {};
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = fmaf(row[i * step + lane + 32 * e], f, o[e]);
+    for (int k = 0; k < JOIN_WARP; ++k) {
+        row[k] = work + ((size_t)b * split * PAIRS + min(m0 + k, j.pairs - 1)) * (HD + 4);
+        end[k] = lane < j.pieces ? *reinterpret_cast<const float2 *>(row[k] + lane * step + HD) : make_float2(-INFINITY, 0.0f);
     }
-    const int group = u.heads / c.kvh, pair = j.m0 + m, tok = pair / group;
-    T *dst = static_cast<T *>(u.out) + ((size_t)(j.r0 + tok) * u.heads + j.h * group + pair - tok * group) * HD;
+    float f[JOIN_WARP], sum[JOIN_WARP];
 #pragma unroll
-    for (int e = 0; e < E; ++e) dst[lane + 32 * e] = from_f<T>(sum == 0.0f ? 0.0f : o[e] / sum);
+    for (int k = 0; k < JOIN_WARP; ++k) {
+        float top = end[k].x;
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
+        f[k] = ex2(end[k].x - (top == -INFINITY ? 0.0f : top));
+        sum[k] = smc_group_sum<32>(lane < j.pieces ? end[k].y * f[k] : 0.0f);
+    }
+#pragma unroll 2
+    for (int i = 0; i < j.pieces; ++i)
+#pragma unroll
+        for (int k = 0; k < JOIN_WARP; ++k) {
+            const float w = __shfl_sync(0xFFFFFFFFu, f[k], i);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[k][e] = fmaf(row[k][i * step + lane + 32 * e], w, o[k][e]);
+        }
+#pragma unroll
+    for (int k = 0; k < JOIN_WARP; ++k) {
+        const int pair = j.m0 + m0 + k, tok = pair / group;
+        if (m0 + k >= j.pairs) break;
+        T *dst = static_cast<T *>(u.out) + ((size_t)(j.r0 + tok) * u.heads + j.h * group + pair - tok * group) * HD;
+#pragma unroll
+        for (int e = 0; e < E; ++e) dst[lane + 32 * e] = from_f<T>(sum[k] == 0.0f ? 0.0f : o[k][e] / sum[k]);
+    }
 }
 
 // jobs of a call (some may be empty: a sequence's share is rounded up), and into how many pieces each one's keys go
@@ -584,7 +638,7 @@ long long items_of(int batch, int rows, int group) { return (long long)rows * gr
 int split_of(const smc_ctx *ctx, int kvh, int batch, int rows, int group, int max_len)
 {
     const long long jobs = items_of(batch, rows, group) * kvh;
-    return (int)std::max(1LL, std::min((long long)max_len / 256, (long long)ctx->sm_count / std::max(1LL, jobs)));
+    return (int)std::max(1LL, std::min({(long long)max_len / KT / STEPS_LEAST, SPLIT_SMS * (long long)ctx->sm_count / std::max(1LL, jobs), 32LL}));  // (a lane a piece joins them)
 }
 
 }  // namespace
@@ -601,17 +655,21 @@ int smc_launch_paged_prompt(smc_ctx *ctx, const smc_paged_view &c, const smc_pag
     const long long items = items_of(c.batch, c.rows, group);
     if (items * c.kvh * split * (PAIRS / 8) > 0x7FFFFFFF || (long long)c.rows * group > 0x7FFFFFFF)
         return smc_fail(ctx, SMC_E_UNSUPPORTED, "paged_attention: %d rows of %d sequences in one call", c.rows, c.batch);
-    auto go = [&](auto main, auto join, uint32_t smem) {
+    const long long jobs = items * c.kvh;
+    auto go = [&](auto main, auto few, auto many, uint32_t smem) {
         cudaFuncSetAttribute(main, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        smc_launch_dep(ctx->use_pdl, main, dim3((unsigned)(items * c.kvh * split)), dim3(THREADS), smem, s, c, u, (int)items, split, work, ctx->d_status);
-        if (split > 1) smc_launch_dep(ctx->use_pdl, join, dim3((unsigned)(items * c.kvh * (PAIRS / 8))), dim3(256), 0, s, c, u, (int)items, split, work);
+        smc_launch_dep(ctx->use_pdl, main, dim3((unsigned)(jobs * split)), dim3(THREADS), smem, s, c, u, (int)items, split, work, ctx->d_status);
+        if (split == 1) return;
+        // (a warp a pair while the device takes them all at once)
+        if (jobs * (PAIRS / 8) <= 8LL * ctx->sm_count) smc_launch_dep(ctx->use_pdl, few, dim3((unsigned)(jobs * (PAIRS / 8))), dim3(256), 0, s, c, u, (int)items, split, work);
+        else smc_launch_dep(ctx->use_pdl, many, dim3((unsigned)(jobs * (PAIRS / 32))), dim3(256), 0, s, c, u, (int)items, split, work);
     };
     if (u.bf16)
-        u.hd == 128 ? go(paged_prompt_kernel<bf16, 128>, paged_prompt_join_kernel<bf16, 128>, Shape<128, false>::SMEM)
-                    : go(paged_prompt_kernel<bf16, 64>, paged_prompt_join_kernel<bf16, 64>, Shape<64, false>::SMEM);
+        u.hd == 128 ? go(paged_prompt_kernel<bf16, 128>, paged_prompt_join_kernel<bf16, 128, 1>, paged_prompt_join_kernel<bf16, 128, 4>, Shape<128, false>::SMEM)
+                    : go(paged_prompt_kernel<bf16, 64>, paged_prompt_join_kernel<bf16, 64, 1>, paged_prompt_join_kernel<bf16, 64, 4>, Shape<64, false>::SMEM);
     else
-        u.hd == 128 ? go(paged_prompt_kernel<float, 128>, paged_prompt_join_kernel<float, 128>, Shape<128, true>::SMEM)
-                    : go(paged_prompt_kernel<float, 64>, paged_prompt_join_kernel<float, 64>, Shape<64, true>::SMEM);
+        u.hd == 128 ? go(paged_prompt_kernel<float, 128>, paged_prompt_join_kernel<float, 128, 1>, paged_prompt_join_kernel<float, 128, 4>, Shape<128, true>::SMEM)
+                    : go(paged_prompt_kernel<float, 64>, paged_prompt_join_kernel<float, 64, 1>, paged_prompt_join_kernel<float, 64, 4>, Shape<64, true>::SMEM);
     SMC_LAUNCH_CHECK(ctx);
     return SMC_OK;
 }
