@@ -510,6 +510,7 @@ size_t smc_paged_decode_work(const smc_ctx *ctx, int kvh, int batch, int heads, 
 int smc_launch_paged_decode(smc_ctx *ctx, const smc_paged_view &c, const smc_paged_query &u, float *work, cudaStream_t s)
 {
     const int pairs = u.max_rows * (u.heads / c.kvh), runs = runs_for(ctx, c.kvh, c.batch, u.max_len);
+    if ((long long)c.batch * c.kvh * pairs > 0x7FFFFFFF) return smc_fail(ctx, SMC_E_UNSUPPORTED, "paged_attention: %d sequences of %d heads in one call", c.batch, u.heads);
     const bool whole = alone(u.max_len), many = (long long)c.batch * c.kvh * pairs >= 1024;  // (many rows to join have few runs each)
     auto pick = [&](auto type, auto hd) {
         using T = decltype(type);

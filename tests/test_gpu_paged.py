@@ -322,6 +322,46 @@ def test_batches_whose_work_is_asked_for(cuda, dtype, heads, kvh, dim):
     assert cuda.device_status() == 0
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [1, 60])
+@pytest.mark.parametrize("scale", [0.0, -0.3, 3.0])
+def test_other_scales(cuda, dtype, rows, scale):
+    """Nothing but the mean, the order turned round, and a sharp softmax; among queries a row of zeros, tiny ones and large ones."""
+    lens = [333, 64]
+    p = Pair(cuda, lens, dim=64, page=16)
+    p.fill(lens)
+    q = randn((2 * rows, 6, 64), "scales", rows)
+    q[0] = 0
+    q[1] *= 1e-30
+    q[-1, 3] *= 1e4
+    q = q.to(dtype)
+    got = p.cache.attention(q.cuda(), p.dtable, ints(lens), scale, row_start=starts([rows, rows]), max_rows=rows)
+    want, bound = paged_util.attention(p.plain, q, p.table, lens, [rows, rows], scale, device="cuda")
+    if scale < 0:  # (the bound's sizes are of the scale's magnitude)
+        bound = paged_util.attention(p.plain, -q, p.table, lens, [rows, rows], -scale, device="cuda")[1]
+    assert bool(((got.cpu().double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("rows", [1, 50])
+def test_a_cache_of_more_than_four_gigabytes(cuda, rows):
+    """Pages whose codes lie behind 2^32 bytes, beside pages in front of them."""
+    kvh, page, dim, pages, heads, length = 8, 64, 128, 68000, 16, 200
+    cache = paged.PagedKVCache.create(cuda, pages, kvh, dim, page)
+    assert cache.k.numel() > 1 << 32
+    plain = paged_util.PlainPages(4, kvh, page, dim)
+    far = ints([[pages - 1, 3, pages - 2, 65536]])
+    k, v = randn((length, kvh, dim), "far k"), randn((length, kvh, dim), "far v")
+    plain.update(k, v, [[0, 1, 2, 3]], [length], [length])
+    cache.Update(k.cuda(), v.cuda(), far, ints([length]), row_start=ints([0, length]))
+    gk, gv = cache.read(far[0])
+    for i in range(3):
+        assert torch.equal(gk[i].cpu(), plain.values(i)[0]) and torch.equal(gv[i].cpu(), plain.values(i)[1])
+    q = randn((rows, heads, dim), "far q")
+    got = cache.attention(q.cuda(), far, ints([length]), 0.1, row_start=None if rows == 1 else ints([0, rows]))
+    want, bound = paged_util.attention(plain, q, [[0, 1, 2, 3]], [length], [rows], 0.1)
+    assert bool(((got.cpu().double() - want).abs() <= bound).all())
+
+
 # ---- where and when it runs
 @pytest.mark.parametrize("rows", [1, 3, 140])
 def test_captured_calls_serve_what_the_arrays_hold(cuda, rows):
@@ -387,6 +427,35 @@ def test_on_another_stream(cuda):
         got = p.cache.attention(q.cuda(non_blocking=False), p.dtable, ints(lens), 0.1)
     side.synchronize()
     near(got, q, p, lens, [1, 1], 0.1)
+
+
+def test_two_threads_on_their_own_streams(cuda):
+    """Calls at the same time, each with its own pages and work space."""
+    import threading
+
+    pairs, wants, faults = [], [], []
+    for i in range(2):
+        p = Pair(cuda, [1200, 300], kvh=4, dim=64, page=32, tag=("thread", i))
+        p.fill([1200, 300], tag=("thread", i))
+        pairs.append((p, randn((2, 16, 64), "t1", i).cuda(), randn((140, 16, 64), "t2", i).cuda(), ints([1200, 300]), ints([0, 100, 140])))
+        wants.append((p.cache.attention(pairs[i][1], p.dtable, pairs[i][3], 0.125), p.cache.attention(pairs[i][2], p.dtable, pairs[i][3], 0.125, row_start=pairs[i][4])))
+    torch.cuda.synchronize()
+
+    def work(i):
+        p, one, many, lens, start = pairs[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                a, b = p.cache.attention(one, p.dtable, lens, 0.125), p.cache.attention(many, p.dtable, lens, 0.125, row_start=start)
+                torch.cuda.current_stream().synchronize()
+                if not (torch.equal(a, wants[i][0]) and torch.equal(b, wants[i][1])):
+                    faults.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not faults
 
 
 # ---- what it refuses
