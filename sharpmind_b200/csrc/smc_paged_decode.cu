@@ -487,15 +487,17 @@ template <int N> struct Dim {
     static constexpr int v = N;
 };
 
-// Up to 8 tiles a segment, two a warp, its CTA goes through it alone and nothing is left to join (16 tiles alone: 18 us from cold caches, spread and joined 9 + 6); else
-// the units are spread evenly, over two CTAs an SM, but four units (one a warp) to each where there are that few.
-constexpr int ALONE = 8;
+// Whole segments to each CTA, and nothing left to join, or the units spread evenly over two CTAs an SM (four units, one a warp, to each where there are that few)?
+// Whole: up to 8 tiles a segment (64 x 8 segments of 8: 18 us, spread 37), and up to 32 where there are four times as many segments (bf16, 4 rows a group, whole /
+// spread: 16 tiles, 16 segments 13.1 / 12.3 us, 32 13.0 / 13.0, 64 13.1 / 17.5, 512 29 / 47; 32 tiles, 16 segments 20 / 13, 128 22 / 37, 512 45 / 55, 1024 81 / 81).
+// Beyond, the longest segments are what the others wait for: 63 tiles, 1024 segments 148 / 123; 125 tiles, 512 segments 152 / 122.
+constexpr int FEW_TILES = 8, SOME_TILES = 32;
 int tiles_of(int max_len) { return std::max(1, (max_len + UNIT - 1) / UNIT); }
-bool alone(int max_len) { return tiles_of(max_len) <= ALONE; }
+bool alone(long long segments, int max_len) { return tiles_of(max_len) <= FEW_TILES || (tiles_of(max_len) <= SOME_TILES && segments >= 4LL * tiles_of(max_len)); }
 int runs_for(const smc_ctx *ctx, int kvh, int batch, int max_len)
 {
     const long long segments = (long long)batch * kvh, most = std::min(2 * ctx->sm_count, RUNS_MOST);
-    return (int)std::min(most, alone(max_len) ? segments : (segments * tiles_of(max_len) + WARPS - 1) / WARPS);
+    return (int)std::min(most, alone(segments, max_len) ? segments : (segments * tiles_of(max_len) + WARPS - 1) / WARPS);
 }
 
 }  // namespace
@@ -504,14 +506,15 @@ bool smc_paged_decode_takes(int group, int max_rows) { return (long long)max_row
 
 size_t smc_paged_decode_work(const smc_ctx *ctx, int kvh, int batch, int heads, int hd, int max_rows, int max_len)
 {
-    return alone(max_len) ? 0 : (size_t)runs_for(ctx, kvh, batch, max_len) * 2 * max_rows * (heads / kvh) * (hd + 4) * sizeof(float);
+    return alone((long long)batch * kvh, max_len) ? 0 : (size_t)runs_for(ctx, kvh, batch, max_len) * 2 * max_rows * (heads / kvh) * (hd + 4) * sizeof(float);
 }
 
 int smc_launch_paged_decode(smc_ctx *ctx, const smc_paged_view &c, const smc_paged_query &u, float *work, cudaStream_t s)
 {
     const int pairs = u.max_rows * (u.heads / c.kvh), runs = runs_for(ctx, c.kvh, c.batch, u.max_len);
     if ((long long)c.batch * c.kvh * pairs > 0x7FFFFFFF) return smc_fail(ctx, SMC_E_UNSUPPORTED, "paged_attention: %d sequences of %d heads in one call", c.batch, u.heads);
-    const bool whole = alone(u.max_len), many = (long long)c.batch * c.kvh * pairs >= 1024;  // (many rows to join have few runs each)
+    // (few rows to join have many runs each: 512 threads a row, 23.3 us for the call of 32 rows over 30 001 keys, 128: 25.4; 2048 rows over 8000: 130 and 121)
+    const bool whole = alone((long long)c.batch * c.kvh, u.max_len), many = (long long)c.batch * c.kvh * pairs >= 1024;
     auto pick = [&](auto type, auto hd) {
         using T = decltype(type);
         constexpr int HD = decltype(hd)::v;

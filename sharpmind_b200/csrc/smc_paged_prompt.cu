@@ -16,7 +16,7 @@
 
 namespace {
 
-constexpr int PAIRS = 256, TILE = 128, KT = 64, G = KT / 16, SOFT_WARPS = 8, CONV_WARP = 8, MMA_WARP = 12, THREADS = 32 * (MMA_WARP + 2), SC_SLOTS = 8, STEPS_LEAST = 4, SPLIT_SMS = 2;  // (a piece of a job has four steps at least, in fp32, whose queries are longer in coming, eight)
+constexpr int PAIRS = 256, TILE = 128, KT = 64, G = KT / 16, SOFT_WARPS = 8, CONV_WARP = 8, MMA_WARP = 12, THREADS = 32 * (MMA_WARP + 2), SC_SLOTS = 8, STEPS_LEAST = 4;
 constexpr float R_BELOW = 6.0f, SUM_MOST = 65000.0f;
 
 // A wait names a phase by its parity: no barrier passes a phase before its waiter has seen the one before.  (PV_DONE may for a softmax, which looks
@@ -633,12 +633,15 @@ __global__ void __launch_bounds__(256) paged_prompt_join_kernel(const smc_paged_
     }
 }
 
-// jobs of a call (some may be empty: a sequence's share is rounded up), and into how many pieces each one's keys go
+// Jobs of a call (some may be empty: a sequence's share is rounded up), and into how many pieces each one's keys go: as many as the device takes at once for one
+// sequence, whose pieces are alike in length (512 bf16 rows behind 5000 keys: 81 us, twice as many 89; 1000 rows 123 / 146; 700 rows the other way, 118 / 110), and
+// twice as many for several of their own lengths (three: 124 us, as many as at once 142, four times as many 142).  A piece has four steps at least (drafts, 8 x 35
+// pairs over 2000 keys: 17.5 us, two 19.9, eight 21.2), in fp32, whose queries are longer in coming, eight.
 long long items_of(int batch, int rows, int group) { return (long long)rows * group / PAIRS + batch; }
 int split_of(const smc_ctx *ctx, int kvh, int batch, int rows, int group, int max_len)
 {
     const long long jobs = items_of(batch, rows, group) * kvh;
-    return (int)std::max(1LL, std::min({(long long)max_len / KT / STEPS_LEAST, SPLIT_SMS * (long long)ctx->sm_count / std::max(1LL, jobs), 32LL}));  // (a lane a piece joins them)
+    return (int)std::max(1LL, std::min({(long long)max_len / KT / STEPS_LEAST, (batch == 1 ? 1LL : 2LL) * ctx->sm_count / std::max(1LL, jobs), 32LL}));  // (a lane a piece joins them)
 }
 
 }  // namespace
@@ -660,7 +663,7 @@ int smc_launch_paged_prompt(smc_ctx *ctx, const smc_paged_view &c, const smc_pag
         cudaFuncSetAttribute(main, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         smc_launch_dep(ctx->use_pdl, main, dim3((unsigned)(jobs * split)), dim3(THREADS), smem, s, c, u, (int)items, split, work, ctx->d_status);
         if (split == 1) return;
-        // (a warp a pair while the device takes them all at once)
+        // (a warp a pair while the device takes them all at once, four else: drafts 17.5 us, the other way 22.1; three prompts 123.5, 126.1)
         if (jobs * (PAIRS / 8) <= 8LL * ctx->sm_count) smc_launch_dep(ctx->use_pdl, few, dim3((unsigned)(jobs * (PAIRS / 8))), dim3(256), 0, s, c, u, (int)items, split, work);
         else smc_launch_dep(ctx->use_pdl, many, dim3((unsigned)(jobs * (PAIRS / 32))), dim3(256), 0, s, c, u, (int)items, split, work);
     };

@@ -303,8 +303,8 @@ def test_prompts_back_to_back(cuda, dtype, heads, dim):
 
 
 @pytest.mark.parametrize("dtype,heads,kvh,dim", [(F32, 8, 8, 64), (BF16, 32, 8, 128), (BF16, 16, 8, 64)])
-def test_batches_whose_work_is_asked_for(cuda, dtype, heads, kvh, dim):
-    """Enough keys for short runs beside the equal ones, lengths far apart, replayed: the same bits each time, whoever took which run."""
+def test_batches_of_lengths_far_apart(cuda, dtype, heads, kvh, dim):
+    """Runs that cut segments and runs that hold many: the same bits each time, with the call's longest length put too short and too long."""
     lens = [20000, 3, 0, 9000, 700, 15000, 64, 5000, 1, 30000]
     p = Pair(cuda, lens, kvh=kvh, dim=dim, page=64, tag="asked")
     p.plain.k[:] = torch.randint(0, 112, p.plain.k.shape, dtype=torch.uint8, generator=gen("codes")) | (torch.randint(0, 2, p.plain.k.shape, dtype=torch.uint8, generator=gen("signs")) << 7)
@@ -319,6 +319,22 @@ def test_batches_whose_work_is_asked_for(cuda, dtype, heads, kvh, dim):
     # shorter and longer than the call says
     for long in (4000, 500000):
         near(p.cache.attention(q.cuda(), p.dtable, ints(lens), dim ** -0.5, max_len=long), q, p, lens, [1] * len(lens), dim ** -0.5)
+    assert cuda.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype,rows,window", [(F32, 1, 0), (BF16, 1, 300), (BF16, 4, 0), (F32, 3, 130)])
+def test_many_segments_of_some_length(cuda, dtype, rows, window):
+    """More segments than blocks of threads on the device, up to 32 tiles each: several whole ones to a block; among them empty sequences and single keys."""
+    lens = [[2048, 0, 1, 700, 1999, 65, 64, 1300][i % 8] for i in range(168)]
+    count = [min(rows, n) for n in lens]
+    p = Pair(cuda, lens, kvh=2, dim=64, page=32, tag="many")
+    p.fill(lens)
+    q = randn((sum(count), 4, 64), "many", rows).to(dtype)
+    start = [0]
+    for n in count:
+        start.append(start[-1] + n)
+    got = p.cache.attention(q.cuda(), p.dtable, ints(lens), 0.125, row_start=ints(start), max_rows=rows, window=window)
+    near(got, q, p, lens, count, 0.125, window)
     assert cuda.device_status() == 0
 
 
