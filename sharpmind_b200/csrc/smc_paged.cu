@@ -386,7 +386,7 @@ int64_t smc_paged_attention_work(smc_ctx *ctx, const smc_paged_kv *kv, int batch
     if (check_cache(ctx, "paged_attention_work", kv, SMC_F32)) return -1;
     if (batch < 0 || rows < 0 || heads <= 0 || heads % kv->kv_heads || max_rows < 0 || max_len < 0) return smc_fail(ctx, -1, "paged_attention_work: bad arguments");
     const int group = heads / kv->kv_heads;
-    return (int64_t)(smc_paged_decode_takes(group, max_rows) ? smc_paged_decode_work(ctx, kv->kv_heads, batch, heads, kv->head_dim, max_rows, max_len)
+    return (int64_t)(smc_paged_decode_takes(group, max_rows, max_len) ? smc_paged_decode_work(ctx, kv->kv_heads, batch, heads, kv->head_dim, max_rows, max_len)
                                                              : smc_paged_prompt_work(ctx, kv->kv_heads, batch, rows, heads, kv->head_dim, max_len));
 }
 
@@ -409,6 +409,6 @@ int smc_paged_attention_dev(smc_ctx *ctx, const smc_paged_kv *kv, const smc_page
     const int64_t need = smc_paged_attention_work(ctx, kv, seqs->batch, seqs->rows, heads, max_rows, max_len);
     if (need > 0 && (!d_work || !aligned(d_work) || work_bytes < need))
         return smc_fail(ctx, SMC_E_INVALID, "paged_attention: %lld bytes of work space are not enough, or not on a 16-byte boundary", work_bytes);
-    if (smc_paged_decode_takes(heads / kv->kv_heads, max_rows)) return smc_launch_paged_decode(ctx, view(kv, seqs), q, static_cast<float *>(d_work), s);
+    if (smc_paged_decode_takes(heads / kv->kv_heads, max_rows, max_len)) return smc_launch_paged_decode(ctx, view(kv, seqs), q, static_cast<float *>(d_work), s);
     return smc_launch_paged_prompt(ctx, view(kv, seqs), q, static_cast<float *>(d_work), s);
 }

@@ -88,7 +88,7 @@ struct smc_paged_query {
     int bf16, heads, hd, window, max_rows, max_len;
     float scale;
 };
-bool smc_paged_decode_takes(int group, int max_rows);
+bool smc_paged_decode_takes(int group, int max_rows, int max_len);
 size_t smc_paged_decode_work(const smc_ctx *, int kvh, int batch, int heads, int hd, int max_rows, int max_len);
 int smc_launch_paged_decode(smc_ctx *, const smc_paged_view &, const smc_paged_query &, float *work, cudaStream_t s);
 size_t smc_paged_prompt_work(const smc_ctx *, int kvh, int batch, int rows, int heads, int hd, int max_len);

@@ -19,7 +19,7 @@
 
 namespace {
 
-constexpr int RUNS_MOST = 1024;
+constexpr int RUNS_MOST = 1024, PART = 16, PARTS_MOST = 4, PART_TILES = 16;
 constexpr int WARPS = 4, THREADS = 32 * WARPS, UNIT = 64, SLOTS = 3, CHUNKS = 256;
 constexpr float W_SHIFT = 14.0f;
 
@@ -59,10 +59,10 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v)
 
 // tiles [t0, t0 + tiles) of 64 keys that rows of sequence s see; one tile, all masked, where there is no key, none where there is no row
 struct Span {
-    int r0, n, len, from, t0, tiles;
+    int r0, n, len, from, t0, tiles, parts;  // parts: its pairs in sixteens
     bool bad;
 };
-__device__ __forceinline__ Span span_of(const smc_paged_view &c, const smc_paged_query &u, int s)
+template <bool PARTED> __device__ __forceinline__ Span span_of(const smc_paged_view &c, const smc_paged_query &u, int s)
 {
     const smc_paged_seq sq = smc_paged_sequence(c, s);
     Span p;
@@ -70,30 +70,33 @@ __device__ __forceinline__ Span span_of(const smc_paged_view &c, const smc_paged
     p.from = u.window > 0 ? max(0, sq.len - p.n + 1 - u.window) : 0;
     p.t0 = p.from / UNIT;
     p.tiles = p.n == 0 ? 0 : max(1, (sq.len + UNIT - 1) / UNIT - p.t0);
+    p.parts = PARTED ? (p.n * (u.heads / c.kvh) + PART - 1) / PART : 1;
     return p;
 }
 // run of units of CTA i of n: [first, first of the next)
 __device__ __forceinline__ int run_first(int i, int n, int units) { return (int)((long long)i * units / n); }
 __device__ __forceinline__ int run_of(int unit, int n, int units) { return (int)(((long long)(unit + 1) * n - 1) / units); }
 
-// Where a warp is among the units: sequence s has [base, base + kvh * tiles)
+// units of a sequence: those of a head's parts follow one another, so that the next part finds the keys in L2
+template <bool PARTED> __device__ __forceinline__ int units_of(const smc_paged_view &c, const Span &p) { return (PARTED ? c.kvh * p.parts : c.kvh) * p.tiles; }
+// Where a warp is among the units: sequence s has [base, base + units_of)
 struct Place {
     int s, base;
     Span p;
 };
-__device__ __forceinline__ void advance(const smc_paged_view &c, const smc_paged_query &u, Place &w, int unit)
+template <bool PARTED> __device__ __forceinline__ void advance(const smc_paged_view &c, const smc_paged_query &u, Place &w, int unit)
 {
-    while (w.base + c.kvh * w.p.tiles <= unit && w.s + 1 < c.batch) {
-        w.base += c.kvh * w.p.tiles;
-        w.p = span_of(c, u, ++w.s);
+    while (w.base + units_of<PARTED>(c, w.p) <= unit && w.s + 1 < c.batch) {
+        w.base += units_of<PARTED>(c, w.p);
+        w.p = span_of<PARTED>(c, u, ++w.s);
     }
 }
 
 // slot of a CTA's cut segment: 0 where it began before the run, 1 where it begins in it
 __device__ __forceinline__ float *partial(float *work, int cta, int which, int rows, int hd) { return work + ((size_t)cta * 2 + which) * rows * (hd + 4); }
 
-// NQ: (row, query head) pairs in eights
-template <typename T, int HD, int NQ>
+// NQ: (row, query head) pairs in eights; PARTED: segments of sixteen pairs each, as many as a sequence's rows need
+template <typename T, int HD, int NQ, bool PARTED>
 __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_paged_view c, const smc_paged_query u, float *work, int aligned, int *status)
 {
     constexpr bool SPLIT = sizeof(T) == 4;  // queries and weights as hi + lo
@@ -119,8 +122,8 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
     for (int i = 0; i < 2; ++i) {
         int n = 0;
         for (int s = (2 * (int)threadIdx.x + i) * per, e = min(c.batch, s + per); s < e; ++s) {
-            const Span p = span_of(c, u, s);
-            n += c.kvh * p.tiles;
+            const Span p = span_of<PARTED>(c, u, s);
+            n += units_of<PARTED>(c, p);
             if (p.bad && blockIdx.x == 0) *status = SMC_STATUS_PAGED;
         }
         mine[i] = n, local += n;
@@ -147,8 +150,8 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
             const int s1 = (int)(segment / c.kvh), g0 = s1 / per;
             if (s1 >= c.batch) return units;
             int before = plan[g0];
-            for (int s = g0 * per; s < s1; ++s) before += c.kvh * span_of(c, u, s).tiles;
-            return before + (int)(segment - (long long)s1 * c.kvh) * span_of(c, u, s1).tiles;
+            for (int s = g0 * per; s < s1; ++s) before += units_of<PARTED>(c, span_of<PARTED>(c, u, s));
+            return before + (int)(segment - (long long)s1 * c.kvh) * (units_of<PARTED>(c, span_of<PARTED>(c, u, s1)) / c.kvh);
         };
         const long long segments = (long long)c.batch * c.kvh;
         first = unit_of(blockIdx.x * segments / gridDim.x), last = unit_of((blockIdx.x + 1) * segments / gridDim.x);
@@ -167,8 +170,8 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
             else hi = mid;
         }
         // (groups behind the last sequence start at `units`)
-        at.s = min(lo * per, c.batch - 1), at.base = plan[lo], at.p = span_of(c, u, at.s);
-        advance(c, u, at, first);
+        at.s = min(lo * per, c.batch - 1), at.base = plan[lo], at.p = span_of<PARTED>(c, u, at.s);
+        advance<PARTED>(c, u, at, first);
     }
 
     // ---- what is on its way: half-stages K, V of this warp's units first + warp, + 4, ...
@@ -180,9 +183,9 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
     auto look = [&](int unit) {
         Fetch f{0, 0, -1, 0, 0};
         if (unit >= last) return f;
-        advance(c, u, ahead, unit);
-        const int rest = unit - ahead.base, h = rest / ahead.p.tiles;
-        f.h = h, f.tile0 = (ahead.p.t0 + rest - h * ahead.p.tiles) * UNIT;
+        advance<PARTED>(c, u, ahead, unit);
+        const int rest = unit - ahead.base, hp = rest / ahead.p.tiles;
+        f.h = PARTED ? hp / ahead.p.parts : hp, f.tile0 = (ahead.p.t0 + rest - hp * ahead.p.tiles) * UNIT;
         f.lo = ahead.p.from, f.hi = ahead.p.len;
         const int key = f.tile0 + 16 * g16, p0 = key >> c.shift << c.shift;
         if (p0 + page > f.lo && p0 < f.hi) {  // (pages that left the window may have gone to another sequence)
@@ -216,16 +219,16 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
 
     // ---- segments
     for (int seg = first; seg < last;) {
-        advance(c, u, at, seg);
+        advance<PARTED>(c, u, at, seg);
         const Span p = at.p;
-        const int h = (seg - at.base) / p.tiles, begin = at.base + h * p.tiles, end = begin + p.tiles, stop = min(end, last);
-        const int pairs = p.n * group;
+        const int hp = (seg - at.base) / p.tiles, begin = at.base + hp * p.tiles, end = begin + p.tiles, stop = min(end, last);
+        const int h = PARTED ? hp / p.parts : hp, m0 = PARTED ? (hp - h * p.parts) * PART : 0, all_pairs = p.n * group, pairs = PARTED ? min(PART, all_pairs - m0) : all_pairs;
         uint32_t q[NQ][PL][KS][2];
         float rowf[NQ][2];  // of rows 2 t, 2 t + 1 of an eight, like all that follows
         int pos[NQ][2];
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq) {
-            const int m = min(8 * nq + g, pairs - 1), i = m / group;  // (rows behind the last repeat it and are not stored)
+            const int m = min(m0 + 8 * nq + g, all_pairs - 1), i = m / group;  // (rows behind the last repeat it and are not stored)
             const T *src = static_cast<const T *>(u.q) + (long long)(p.r0 + i) * u.q_stride + (size_t)(h * group + m - i * group) * HD + 16 * t;
             float x[4 * KS], most = 0.0f;
 #pragma unroll
@@ -248,7 +251,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 rowf[nq][e] = __shfl_sync(0xFFFFFFFFu, back, 4 * (2 * t + e));
-                pos[nq][e] = p.len - p.n + min(8 * nq + 2 * t + e, pairs - 1) / group;
+                pos[nq][e] = p.len - p.n + min(m0 + 8 * nq + 2 * t + e, all_pairs - 1) / group;
             }
         }
         float o[NQ][KS][4] = {}, M[NQ][2], l[NQ][2];
@@ -384,7 +387,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     const float *rows = merge + (2 * warp + r) * R::MERGE_ROW;  // of warp v: + 8 v rows
-                    const int m = 8 * nq + 2 * warp + r, tok = m / group;
+                    const int m = 8 * nq + 2 * warp + r, pair = m0 + m, tok = pair / group;
                     if (m >= pairs) continue;
                     float top = -INFINITY, fac[WARPS], all = 0.0f;
 #pragma unroll
@@ -396,8 +399,8 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
                         all = fmaf(rows[v * 8 * R::MERGE_ROW + HD / 2 + 1], fac[v], all);
                     }
                     const float norm = whole ? (all == 0.0f ? 0.0f : 1.0f / all) : 1.0f;
-                    float *part_row = partial(work, blockIdx.x, begin < first ? 0 : 1, u.max_rows * group, HD) + (size_t)m * (HD + 4);
-                    T *dst = static_cast<T *>(u.out) + ((size_t)(p.r0 + tok) * u.heads + h * group + m - tok * group) * HD;
+                    float *part_row = partial(work, blockIdx.x, begin < first ? 0 : 1, PARTED ? PART : u.max_rows * group, HD) + (size_t)m * (HD + 4);
+                    T *dst = static_cast<T *>(u.out) + ((size_t)(p.r0 + tok) * u.heads + h * group + pair - tok * group) * HD;
 #pragma unroll
                     for (int i = 0; i < HD / 64; ++i) {
                         float a = 0.0f;
@@ -417,7 +420,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
 
 // One block of threads = one row and head: joins what the runs left of its segment.  Four dimensions a thread, the runs dealt to groups of threads, so that
 // all loads go out at once; each group adds its runs in their order, then the groups' sums are added in theirs.
-template <typename T, int HD, int JOIN_THREADS>
+template <typename T, int HD, int JOIN_THREADS, bool PARTED>
 __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const smc_paged_view c, const smc_paged_query u, const float *__restrict__ work, int grid)
 {
     constexpr int LANES = HD / 4, GROUPS = JOIN_THREADS / LANES;
@@ -428,7 +431,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const smc_page
     __shared__ float4 outs[GROUPS][LANES];
     int before = 0, units = 0;
     for (int i = tid; i < c.batch; i += JOIN_THREADS) {
-        const int n = c.kvh * span_of(c, u, i).tiles;
+        const int n = units_of<PARTED>(c, span_of<PARTED>(c, u, i));
         units += n;
         if (i < s) before += n;
     }
@@ -438,11 +441,11 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const smc_page
     before = 0, units = 0;
 #pragma unroll
     for (int i = 0; i < JOIN_THREADS / 32; ++i) before += part[0][i], units += part[1][i];
-    const Span p = span_of(c, u, s);
+    const Span p = span_of<PARTED>(c, u, s);
     if (m >= p.n * group) return;
-    const int runs = min(grid, units), begin = before + h * p.tiles, c0 = run_of(begin, runs, units), count = run_of(begin + p.tiles - 1, runs, units) - c0 + 1;
+    const int runs = min(grid, units), begin = before + (PARTED ? h * p.parts + m / PART : h) * p.tiles, c0 = run_of(begin, runs, units), count = run_of(begin + p.tiles - 1, runs, units) - c0 + 1;
     if (count == 1) return;  // whole in one run
-    auto row = [&](int i) { return work + ((size_t)(c0 + i) * 2 + (i == 0)) * most * (HD + 4) + (size_t)m * (HD + 4); };
+    auto row = [&](int i) { return work + ((size_t)(c0 + i) * 2 + (i == 0)) * (PARTED ? PART : most) * (HD + 4) + (size_t)(PARTED ? m % PART : m) * (HD + 4); };
     float top = -INFINITY, sum_mine = 0.0f;
     for (int i = tid; i < count; i += JOIN_THREADS) {
         factor[i] = row(i)[HD];
@@ -492,42 +495,55 @@ template <int N> struct Dim {
 // spread: 16 tiles, 16 segments 13.1 / 12.3 us, 32 13.0 / 13.0, 64 13.1 / 17.5, 512 29 / 47; 32 tiles, 16 segments 20 / 13, 128 22 / 37, 512 45 / 55, 1024 81 / 81).
 // Beyond, the longest segments are what the others wait for: 63 tiles, 1024 segments 148 / 123; 125 tiles, 512 segments 152 / 122.
 constexpr int FEW_TILES = 8, SOME_TILES = 32;
-int tiles_of(int max_len) { return std::max(1, (max_len + UNIT - 1) / UNIT); }
+int tiles_of(int max_len) { return max_len <= 0 ? 1 : (max_len - 1) / UNIT + 1; }
 bool alone(long long segments, int max_len) { return tiles_of(max_len) <= FEW_TILES || (tiles_of(max_len) <= SOME_TILES && segments >= 4LL * tiles_of(max_len)); }
-int runs_for(const smc_ctx *ctx, int kvh, int batch, int max_len)
+int parts_of(int pairs) { return (pairs + PART - 1) / PART; }
+int runs_for(const smc_ctx *ctx, int kvh, int batch, int parts, int max_len)
 {
     const long long segments = (long long)batch * kvh, most = std::min(2 * ctx->sm_count, RUNS_MOST);
-    return (int)std::min(most, alone(segments, max_len) ? segments : (segments * tiles_of(max_len) + WARPS - 1) / WARPS);
+    return (int)std::min(most, alone(segments, max_len) ? segments : (segments * parts * tiles_of(max_len) + WARPS - 1) / WARPS);
 }
 
 }  // namespace
 
-bool smc_paged_decode_takes(int group, int max_rows) { return (long long)max_rows * group <= 16; }
+// A part costs a pass over the keys, from L2 but for the first, where the tcgen05 form takes 256 pairs at once: up to four parts, and sixteen tiles of keys for each
+// (bf16, here / there: 20 pairs, 64 sequences of up to 8000 keys 259 / 555 us, of up to 2000 108 / 157, one of 500 19 / 16; 35 pairs, 64 of 2000 57 / 49, of 3000
+// 60 / 73; 64 pairs, 64 of 3000 258 / 224, of 4000 254 / 276, of 8000 336 / 524).  Up to 16 pairs: 16, one sequence of 500 12 / 16 us, 64 of 8000 151 / 523.
+bool smc_paged_decode_takes(int group, int max_rows, int max_len)
+{
+    const long long pairs = (long long)max_rows * group;
+    return pairs <= PART || (pairs <= PART * PARTS_MOST && tiles_of(max_len) >= PART_TILES * (int)((pairs + PART - 1) / PART));
+}
 
 size_t smc_paged_decode_work(const smc_ctx *ctx, int kvh, int batch, int heads, int hd, int max_rows, int max_len)
 {
-    return alone((long long)batch * kvh, max_len) ? 0 : (size_t)runs_for(ctx, kvh, batch, max_len) * 2 * max_rows * (heads / kvh) * (hd + 4) * sizeof(float);
+    return alone((long long)batch * kvh, max_len) ? 0 : (size_t)runs_for(ctx, kvh, batch, parts_of(max_rows * (heads / kvh)), max_len) * 2 * std::min(PART, max_rows * (heads / kvh)) * (hd + 4) * sizeof(float);
 }
 
 int smc_launch_paged_decode(smc_ctx *ctx, const smc_paged_view &c, const smc_paged_query &u, float *work, cudaStream_t s)
 {
-    const int pairs = u.max_rows * (u.heads / c.kvh), runs = runs_for(ctx, c.kvh, c.batch, u.max_len);
-    if ((long long)c.batch * c.kvh * pairs > 0x7FFFFFFF) return smc_fail(ctx, SMC_E_UNSUPPORTED, "paged_attention: %d sequences of %d heads in one call", c.batch, u.heads);
+    const int pairs = u.max_rows * (u.heads / c.kvh), runs = runs_for(ctx, c.kvh, c.batch, parts_of(pairs), u.max_len);
+    const long long capacity = ((long long)c.width << c.shift) / UNIT + 2;  // (tiles that a sequence may have)
+    if (capacity * parts_of(pairs) > 0x7FFFFFFF / ((long long)c.batch * c.kvh) || (long long)c.batch * c.kvh * pairs > 0x7FFFFFFF) return smc_fail(ctx, SMC_E_UNSUPPORTED, "paged_attention: %d sequences of %d heads in one call", c.batch, u.heads);
     // (few rows to join have many runs each: 512 threads a row, 23.3 us for the call of 32 rows over 30 001 keys, 128: 25.4; 2048 rows over 8000: 130 and 121)
     const bool whole = alone((long long)c.batch * c.kvh, u.max_len), many = (long long)c.batch * c.kvh * pairs >= 1024;
-    auto pick = [&](auto type, auto hd) {
+    auto pick = [&](auto type, auto hd, auto parted) {
         using T = decltype(type);
         constexpr int HD = decltype(hd)::v;
-        auto main = pairs <= 8 ? paged_decode_kernel<T, HD, 1> : paged_decode_kernel<T, HD, 2>;
+        constexpr bool PARTED = decltype(parted)::v != 0;
+        auto main = paged_decode_kernel<T, HD, 2, PARTED>;
+        if constexpr (!PARTED)
+            if (pairs <= 8) main = paged_decode_kernel<T, HD, 1, false>;
         cudaFuncSetAttribute(main, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<HD>::SMEM);
         smc_launch_dep(ctx->use_pdl, main, dim3(runs), dim3(THREADS), Ring<HD>::SMEM, s, c, u, work, whole ? 1 : 0, ctx->d_status);
         if (whole || runs == 1) return;
         const dim3 grid((unsigned)(c.batch * c.kvh * pairs));
-        if (many) smc_launch_dep(ctx->use_pdl, paged_join_kernel<T, HD, 128>, grid, dim3(128), 0, s, c, u, work, runs);
-        else smc_launch_dep(ctx->use_pdl, paged_join_kernel<T, HD, 512>, grid, dim3(512), 0, s, c, u, work, runs);
+        if (many) smc_launch_dep(ctx->use_pdl, paged_join_kernel<T, HD, 128, PARTED>, grid, dim3(128), 0, s, c, u, work, runs);
+        else smc_launch_dep(ctx->use_pdl, paged_join_kernel<T, HD, 512, PARTED>, grid, dim3(512), 0, s, c, u, work, runs);
     };
-    if (u.bf16) u.hd == 128 ? pick(bf16(), Dim<128>()) : pick(bf16(), Dim<64>());
-    else u.hd == 128 ? pick(float(), Dim<128>()) : pick(float(), Dim<64>());
+    auto form = [&](auto type, auto hd) { pairs > PART ? pick(type, hd, Dim<1>()) : pick(type, hd, Dim<0>()); };
+    if (u.bf16) u.hd == 128 ? form(bf16(), Dim<128>()) : form(bf16(), Dim<64>());
+    else u.hd == 128 ? form(float(), Dim<128>()) : form(float(), Dim<64>());
     SMC_LAUNCH_CHECK(ctx);
     return SMC_OK;
 }

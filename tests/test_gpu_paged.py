@@ -339,6 +339,27 @@ def test_many_segments_of_some_length(cuda, dtype, rows, window):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("kvh,most,batch,window", [(2, 5, 6, 0), (1, 16, 7, 0), (2, 9, 5, 700), (2, 5, 72, 0), (1, 12, 160, 0)])
+def test_drafts_over_long_caches(cuda, dtype, dim, kvh, most, batch, window):
+    """17 to 64 (row, head) pairs of a sequence, beside sequences with fewer and with none; long enough for the form that takes them in sixteens."""
+    lens = [[4500, 70, 1025, 0, 2000, 3, 4096][i % 7] for i in range(batch)]
+    count = [min([most, 1, most - 1, 3, 0, 2][i % 6], n) for i, n in enumerate(lens)]
+    p = Pair(cuda, lens, kvh=kvh, dim=dim, page=32, tag="drafts")
+    p.fill(lens)
+    group = 4
+    q = randn((sum(count), kvh * group, dim), "drafts", most).to(dtype)
+    args = dict(row_start=starts(count), max_rows=most, window=window)
+    got = p.cache.attention(q.cuda(), p.dtable, ints(lens), dim ** -0.5, **args)
+    near(got, q, p, lens, count, dim ** -0.5, window)
+    assert torch.equal(got, p.cache.attention(q.cuda(), p.dtable, ints(lens), dim ** -0.5, **args))
+    # a longest length that says less than there is, and so the forms for shorter ones; one that says all that there may be
+    for long in (600, 2048, 2 ** 31 - 1):
+        near(p.cache.attention(q.cuda(), p.dtable, ints(lens), dim ** -0.5, max_len=long, **args), q, p, lens, count, dim ** -0.5, window)
+    assert cuda.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("rows", [1, 60])
 @pytest.mark.parametrize("scale", [0.0, -0.3, 3.0])
 def test_other_scales(cuda, dtype, rows, scale):
