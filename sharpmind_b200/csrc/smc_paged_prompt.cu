@@ -11,6 +11,8 @@
 // Warp roles:  0 .. 3, 4 .. 7  softmax of tile 0, 1      8 .. 11  codes to fp16      12, 13  MMA issue of tile 0, 1
 // Scores have two buffers a tile, so a softmax finds its next ones there.
 // Few pairs: the steps are split over CTAs, whose partial results a second kernel joins.
+// Measured (6000 bf16 rows, 32 query heads, 8 of keys, of 128): 391 us, 754 TFLOP/s, 45 % of a bf16 matmul's rate; 1.46 us a step.  Tensor pipe 30 % active, issue slots 42 %: the chain from scores to weights
+// bounds it, no unit.  Leaving out the exponentials gained 1 %, all MMAs 7 %, the stores of the converted tiles 11 %.
 #include "smc_paged.cuh"
 #include "smc_tc.cuh"
 
@@ -25,7 +27,7 @@ enum { FULL = 0, EMPTY = 4, S_FULL = 8, P_FULL = 12 /* [tile][step parity] */, P
 
 template <int HD, bool SPLIT>
 struct Shape {
-    static constexpr int PLANES = SPLIT ? 2 : 1, STAGES = 2;  // (each stage has its own copy of the MMAs: four were slower, the SM's instruction cache has enough to hold)
+    static constexpr int PLANES = SPLIT ? 2 : 1, STAGES = 2;  // (each stage has its own copy of the MMAs: four took 398 us where two take 392, 6000 rows)
     static constexpr uint32_t SUB_Q = TILE * 128, Q_PLANE = HD / 64 * SUB_Q, Q_TILE = PLANES * Q_PLANE;
     static constexpr uint32_t HALF = KT * HD * 2, STAGE = 2 * HALF;  // fp16 keys of a step, values of the last step but one
     static constexpr uint32_t OFF_K = 2 * Q_TILE, OFF_SC = OFF_K + STAGES * STAGE, OFF_BAR = OFF_SC + SC_SLOTS * G * 16, SMEM = OFF_BAR + 256;
@@ -587,7 +589,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
     }
 }
 
-// One warp = JOIN_WARP pairs of a job whose keys were split: joins the pieces in their order.
+// One warp = JOIN_WARP pairs of a job whose keys were split: joins the pieces in their order.  Latency and L2 bound it: drafts' 576 blocks 7.4 us, three prompts' 1024 19 (cold caches).
 template <typename T, int HD, int JOIN_WARP>
 __global__ void __launch_bounds__(256) paged_prompt_join_kernel(const smc_paged_view c, const smc_paged_query u, int items, int split, const float *__restrict__ work)
 {
