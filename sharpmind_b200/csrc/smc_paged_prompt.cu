@@ -117,8 +117,8 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b)
 __device__ __forceinline__ int row_shift(float most) { return min(14 - ((int)(__float_as_uint(most) >> 23) - 127), 126); }
 __host__ __device__ constexpr uint32_t idesc_f16(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TILE >> 4) << 24); }
 
-// One thread issues a tile's MMAs: at step x, O += P(x - 2) V(x - 2) and the scores of x.  These take the columns that P(x - 2) is in: the MMAs of a thread run in
-// their order (checked: weights overwritten by the next product's scores at once, 30 000 times).
+// One thread issues a tile's MMAs: at step x, O += P(x - 2) V(x - 2) and the scores of x.  These take the columns that P(x - 2) is in.  Only MMAs of one accumulator
+// and shape are promised to run in their order, so the scores wait until the product has completed; the softmax of x - 1 runs meanwhile.
 template <int HD, bool SPLIT, int TILE_NO>
 __device__ __forceinline__ void issue_mmas(uint32_t sbase, int mine, int n, uint32_t bars, volatile uint32_t *abort_flag, int *status)
 {
@@ -144,6 +144,10 @@ __device__ __forceinline__ void issue_mmas(uint32_t sbase, int mine, int n, uint
             if (x - 1 == mine) smc_tc_commit(bar(O_FULL + TILE_NO));
         }
         if (x < mine) {
+            if (x >= 2) {
+                wait(PV_DONE + TILE_NO, (uint32_t)(x - 2));
+                smc_tc_fence_after();
+            }
             each<S::PLANES * (HD / 16)>([&](auto i) {
                 constexpr int p = S::PLANES - 1 - decltype(i)::v / (HD / 16), ks = decltype(i)::v % (HD / 16);
                 mma_ss<S::COL_S + (2 * TILE_NO + st % 2) * KT, TILE_NO * S::Q_TILE + p * S::Q_PLANE + ks / 4 * S::SUB_Q + ks % 4 * 32,
