@@ -75,6 +75,17 @@ __device__ __forceinline__ uint32_t smc_float_e4m3x4(const float (&f)[4])
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b) : "f"(f[3]), "f"(f[2]));
     return (uint32_t)a | ((uint32_t)b << 16);
 }
+// A weight carries its value's scale, w = 2^(y - R), y = x + log2 s_v, and the softmax's sum is l = sum 2^(x - R) = sum w / s_v.  Scales are 2^-40 .. 2^120 and the
+// largest y is at most 16 above R, so of the keys of a row the one with the largest x has 2^(x - R) >= 2^-120, while its w, and the factor that brings an earlier sum
+// to a new R, may be smaller than fp32 holds (2^-126): both attention forms keep the sum from losing it.
+__device__ __forceinline__ int smc_paged_log2(float scale) { return (int)(__float_as_uint(scale) >> 23) - 127; }  // of a power of two; 128 of an undefined one
+// l 2^d + add for d <= 0; 2^d itself may vanish where l 2^d counts
+__device__ __forceinline__ float smc_paged_fold(float l, float d, float add)
+{
+    float f = ex2(d);
+    if (d < -100.0f) f = ex2(0.5f * d), l *= f;
+    return fmaf(l, f, add);
+}
 // Four neighbouring elements of a row as floats, and floats as elements
 template <typename T> __device__ __forceinline__ void smc_paged_load4(const T *p, float (&f)[4]) { load_v<T, 4>(p, f); }
 template <typename T> __device__ __forceinline__ void smc_paged_store4(T *p, const float (&f)[4]) { store_v<T, 4>(p, f); }

@@ -16,7 +16,9 @@
 // the keys, tokens [16 t, 16 t + 16) of the values.  The scores' row i of tile pair M is token 16 (i / 2) + 2 M + i % 2: a transposed eight by eight
 // block of weights (movmatrix) then is the second product's operand, and all tokens of a thread's scores lie in one page, so a unit's scales are two numbers.
 //   y_j = x_j log2(e) + log2(s_v);  w_j = 2^(y_j - M), M the running maximum of y less 14;  O = sum w_j code_j;  l = sum w_j / s_v;  out = O / l
-// The value scales ride in the exponent, so the weights stay within fp16 whatever the scales are: 2^14 at most, and 2^-38 of that still counts.
+// The value scales ride in the exponent, so the weights stay within fp16: 2^14 at most, in steps of 2^-24 at least (fp32: hi and lo together), 2^-38 of the largest.
+// The sum takes every key whatever the scales are: a thread whose keys' weights all lie below 2^-60, 0 as fp16 numbers, takes them 2^64 up (scales are 2^-40 .. 2^120, so a
+// weight may be 2^-150 and count).  That and the sums' way to a new M are worth 0.1 to 0.6 us of a step of single tokens, 4 of 151 for 4 rows over 64 sequences of up to 8000.
 #include "smc_async.cuh"
 #include "smc_paged.cuh"
 
@@ -24,7 +26,7 @@ namespace {
 
 constexpr int RUNS_MOST = 1024, PART = 16, PARTS_MOST = 4, PART_TILES = 16;
 constexpr int WARPS = 4, THREADS = 32 * WARPS, UNIT = 64, SLOTS = 3, CHUNKS = 256;
-constexpr float W_SHIFT = 14.0f;
+constexpr float W_SHIFT = 14.0f, W_UP = 64.0f, W_DOWN = 0x1p-64f, LOW = -60.0f;
 
 template <int HD>
 struct Ring {
@@ -266,7 +268,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
             later = look(unit + 2 * WARPS);
             sc_next = scales_of(next);
             // (a power of two's exponent; a scale that is none, left where no page is or undefined, stays what it is)
-            const float bias = sc_now.y == sc_now.y ? (float)((int)(__float_as_uint(sc_now.y) >> 23) - 127) : sc_now.y, inv = 1.0f / sc_now.y;
+            const float bias = sc_now.y == sc_now.y ? (float)smc_paged_log2(sc_now.y) : sc_now.y, inv = 1.0f / sc_now.y;
             const bool inner = now.tile0 >= now.lo && now.tile0 + UNIT <= p.len - p.n + 1 && (u.window <= 0 || now.tile0 > p.len - 1 - u.window);
             landed(half);
             float s[NQ][4][4] = {};
@@ -294,7 +296,8 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
             uint32_t w[NQ][PL][8];  // weights as B fragments: block M of tokens
 #pragma unroll
             for (int nq = 0; nq < NQ; ++nq) {
-                float corr[2];
+                float down[2], add[2];
+                uint32_t seen = 0;  // ones where a row's weights are not 2^W_UP up
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     const float f = rowf[nq][r] * sc_now.x;
@@ -309,28 +312,35 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
                     float top = s[nq][0][r];
 #pragma unroll
                     for (int j = 1; j < 8; ++j) top = fmaxf(top, s[nq][j >> 1][2 * (j & 1) + r]);
+                    const float mine = top;
                     top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
                     top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
                     top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
                     const float nm = fmaxf(M[nq][r], top - W_SHIFT), ref = nm == -INFINITY ? 0.0f : nm;
-                    corr[r] = ex2(M[nq][r] - ref);  // (-inf: nothing yet, 0)
+                    down[r] = M[nq][r] - ref;  // (-inf: nothing yet)
                     M[nq][r] = nm;
+                    const bool low = mine - ref < LOW;
+                    const float from = low ? ref - W_UP : ref;
+                    seen |= low ? 0u : 0xFFFFu << (16 * r);
                     float sum = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) sum += s[nq][j >> 1][2 * (j & 1) + r] = ex2(s[nq][j >> 1][2 * (j & 1) + r] - ref);
-                    // (a row that sees none of these tokens takes nothing of their scale, which may be undefined)
-                    l[nq][r] = fmaf(l[nq][r], corr[r], sum == 0.0f ? 0.0f : sum * inv);
+                    for (int j = 0; j < 8; ++j) sum += s[nq][j >> 1][2 * (j & 1) + r] = ex2(s[nq][j >> 1][2 * (j & 1) + r] - from);
+                    // (first by the scale's inverse: neither product leaves fp32.  A row that sees none of these tokens takes nothing of their scale, which may be undefined)
+                    add[r] = sum == 0.0f ? 0.0f : sum * inv * (low ? W_DOWN : 1.0f);
                 }
-                if (__any_sync(0xFFFFFFFFu, corr[0] != 1.0f || corr[1] != 1.0f)) {
+                if (__any_sync(0xFFFFFFFFu, down[0] != 0.0f || down[1] != 0.0f)) {
+                    const float corr[2] = {ex2(down[0]), ex2(down[1])};
+                    l[nq][0] = smc_paged_fold(l[nq][0], down[0], 0.0f), l[nq][1] = smc_paged_fold(l[nq][1], down[1], 0.0f);
 #pragma unroll
                     for (int i = 0; i < KS; ++i) o[nq][i][0] *= corr[0], o[nq][i][1] *= corr[1], o[nq][i][2] *= corr[0], o[nq][i][3] *= corr[1];
                 }
+                l[nq][0] += add[0], l[nq][1] += add[1];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const float a = s[nq][j >> 1][2 * (j & 1)], b = s[nq][j >> 1][2 * (j & 1) + 1];
                     const uint32_t hi = half2_bits(a, b);
-                    w[nq][0][j] = transposed(hi);
-                    if constexpr (SPLIT) w[nq][1][j] = transposed(rest_bits(a, b, hi));
+                    w[nq][0][j] = transposed(hi & seen);
+                    if constexpr (SPLIT) w[nq][1][j] = transposed(rest_bits(a, b, hi) & seen);
                 }
             }
             landed(half);
@@ -398,8 +408,9 @@ __global__ void __launch_bounds__(THREADS, 2) paged_decode_kernel(const smc_page
                     const float ref = top == -INFINITY ? 0.0f : top;
 #pragma unroll
                     for (int v = 0; v < WARPS; ++v) {
-                        fac[v] = ex2(rows[v * 8 * R::MERGE_ROW + HD / 2] - ref);
-                        all = fmaf(rows[v * 8 * R::MERGE_ROW + HD / 2 + 1], fac[v], all);
+                        const float down = rows[v * 8 * R::MERGE_ROW + HD / 2] - ref;
+                        fac[v] = ex2(down);
+                        all = smc_paged_fold(rows[v * 8 * R::MERGE_ROW + HD / 2 + 1], down, all);
                     }
                     const float norm = whole ? (all == 0.0f ? 0.0f : 1.0f / all) : 1.0f;
                     float *part_row = partial(work, blockIdx.x, begin < first ? 0 : 1, PARTED ? PART : u.max_rows * group, HD) + (size_t)m * (HD + 4);
@@ -462,8 +473,9 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const smc_page
     for (int i = 0; i < JOIN_THREADS / 32; ++i) top = fmaxf(top, tops[i]);
     const float ref = top == -INFINITY ? 0.0f : top;
     for (int i = tid; i < count; i += JOIN_THREADS) {
-        factor[i] = ex2(factor[i] - ref);
-        sum_mine = fmaf(row(i)[HD + 1], factor[i], sum_mine);
+        const float down = factor[i] - ref;
+        factor[i] = ex2(down);
+        sum_mine = smc_paged_fold(row(i)[HD + 1], down, sum_mine);
     }
     const float sum_warp = smc_group_sum<32>(sum_mine);
     if ((tid & 31) == 0) sums[tid >> 5] = sum_warp;

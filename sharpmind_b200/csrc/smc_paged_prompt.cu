@@ -20,6 +20,10 @@ namespace {
 
 constexpr int PAIRS = 256, TILE = 128, KT = 64, G = KT / 16, SOFT_WARPS = 8, CONV_WARP = 8, MMA_WARP = 12, THREADS = 32 * (MMA_WARP + 2), SC_SLOTS = 8, STEPS_LEAST = 4;
 constexpr float R_BELOW = 6.0f, SUM_MOST = 65000.0f;
+// A step with a value scale 2^SCALES_NEAR or more below an earlier one takes a pass of its own for the softmax's sum, over 2^(R - SUM_UP).  (Under nearer scales a key that
+// w loses is 2^-68 of a larger one.  The pass is the step's own loop once more: in code of its own it cost every step, 6000 rows 407 us; so, as without it, 392 to 394.)
+constexpr int SCALES_NEAR = 64;
+constexpr float SUM_UP = 48.0f, SUM_DOWN = 0x1p-48f;
 
 // A wait names a phase by its parity: no barrier passes a phase before its waiter has seen the one before.  (PV_DONE may for a softmax, which looks
 // at it only in step i for the product of step i - 1, where neither the one before can be missing nor the one after be there.)
@@ -377,7 +381,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
                 x[k].x = fmaxf(x[k].x * rowf, 1e-37f);
                 if (!inner && (16 * k > hi || 16 * k + 15 <= lo)) x[k].y = -INFINITY, x[k].z = 0.0f;
             }
-            float add;
+            float add, far = x[0].w;
 #pragma unroll 1
             for (bool again = true;;) {
                 const float ref = R == -INFINITY ? 0.0f : R;
@@ -403,7 +407,20 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
                 }
                 // No maximum is taken where the weights' sum tells that none of them is too large.  (A row's first step has no R yet.)
                 const bool bad = again && (R == -INFINITY || total > SUM_MOST);
-                if (!__any_sync(0xFFFFFFFFu, bad)) break;
+                if (!__any_sync(0xFFFFFFFFu, bad || far != 0.0f)) break;
+                if (!__any_sync(0xFFFFFFFFu, bad)) {
+                    if (far == 1.0f) {  // R is this step's from here: a pass for the sum alone
+                        far = 2.0f, again = false;
+#pragma unroll
+                        for (int k = 0; k < G; ++k) x[k].y = x[k].y == -INFINITY ? x[k].y : SUM_UP;
+                    } else {  // and the weights once more, which add nothing to it
+                        l = fmaf(total, SUM_DOWN, l), far = 0.0f;
+#pragma unroll
+                        for (int k = 0; k < G; ++k) x[k].y = x[k].y == -INFINITY ? x[k].y : sc[k].y, x[k].z = 0.0f;
+                    }
+                    tmem_wait_st();
+                    continue;
+                }
                 again = false;
                 tmem_wait_st();
                 float top = -INFINITY;
@@ -415,13 +432,14 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
                         m4[e] = fmaxf(fmaxf(__uint_as_float(s[16 * k + e]), __uint_as_float(s[16 * k + 4 + e])), fmaxf(__uint_as_float(s[16 * k + 8 + e]), __uint_as_float(s[16 * k + 12 + e])));
                     top = fmaxf(top, fmaf(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), x[k].x, x[k].y));  // (what is not a number a maximum drops)
                 }
-                float corr = 1.0f;
+                float down = 0.0f;
                 if (bad && top > -INFINITY) {
                     const float was = R;
                     R = top - R_BELOW;
-                    corr = ex2(was - R);
+                    down = was - R;
                 }
-                l *= corr;
+                const float corr = ex2(down);
+                l = smc_paged_fold(l, down, 0.0f);
                 if (it > 0) {
                     wait(PV_DONE + t, (uint32_t)(it - 1));  // (the one before that: these scores waited for it)
                     smc_tc_fence_after();
@@ -535,6 +553,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
         uint4 raw_k[UNITS], raw_v[UNITS];
         int id_k = page_of(j.i0), id_1 = -1, id_v = -1;  // pages of the keys of step x, of those before, of the values
         float2 sc = scales_of(id_k);
+        int largest = -127;  // log2 of the largest value scale so far
 #pragma unroll
         for (int i = 0; i < UNITS; ++i) raw_k[i] = fetch_k(id_k, i);
 #pragma unroll 1
@@ -562,11 +581,15 @@ __global__ void __launch_bounds__(THREADS, 1) paged_prompt_kernel(const smc_page
 #pragma unroll
             for (int i = 0; i < UNITS; ++i) raw_v[i] = fetch_v(v_page, i);
             if (x < n) {
-                if (w == 0 && lane < G) {
-                    // scale of keys; log2 and reciprocal of that of values (a power of two's exponent).  An undefined one of either makes the second undefined
-                    const float both = sc.x + sc.y, e = (float)((int)(__float_as_uint(sc.y) >> 23) - 127);
-                    reinterpret_cast<float4 *>(smem + S::OFF_SC)[(x % SC_SLOTS) * G + lane] =
-                        id_k < 0 ? make_float4(0.0f, -INFINITY, 0.0f, 0.0f) : make_float4(sc.x, both == both ? e : both, 1.0f / sc.y, 0.0f);
+                if (w == 0) {  // (its lanes have the step's groups of keys, again and again)
+                    // scale of keys; log2 and reciprocal of that of values (a power of two's exponent); 1 where the step's value scales lie far below an earlier one.
+                    // An undefined one of either makes the second undefined
+                    const int log2v = id_k < 0 ? -127 : smc_paged_log2(sc.y);
+                    largest = max(largest, __reduce_max_sync(0xFFFFFFFFu, log2v));
+                    const float both = sc.x + sc.y, e = (float)log2v, far = __any_sync(0xFFFFFFFFu, id_k >= 0 && log2v < largest - SCALES_NEAR) ? 1.0f : 0.0f;
+                    if (lane < G)
+                        reinterpret_cast<float4 *>(smem + S::OFF_SC)[(x % SC_SLOTS) * G + lane] =
+                            id_k < 0 ? make_float4(0.0f, -INFINITY, 0.0f, far) : make_float4(sc.x, both == both ? e : both, 1.0f / sc.y, far);
                 }
 #pragma unroll
                 for (int i = 0; i < UNITS; ++i) place(k_dst + (uint32_t)st * S::STAGE + (uint32_t)(STEP_K * i) * 1024u + swizzle, raw_k[i]);
@@ -618,8 +641,9 @@ __global__ void __launch_bounds__(256) paged_prompt_join_kernel(const smc_paged_
         float top = end[k].x;
 #pragma unroll
         for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
-        f[k] = ex2(end[k].x - (top == -INFINITY ? 0.0f : top));
-        sum[k] = smc_group_sum<32>(lane < j.pieces ? end[k].y * f[k] : 0.0f);
+        const float down = end[k].x - (top == -INFINITY ? 0.0f : top);
+        f[k] = ex2(down);
+        sum[k] = smc_group_sum<32>(lane < j.pieces ? smc_paged_fold(end[k].y, down, 0.0f) : 0.0f);
     }
 #pragma unroll 2
     for (int i = 0; i < j.pieces; ++i)
