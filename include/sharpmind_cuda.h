@@ -376,9 +376,12 @@ SMC_API int smc_sdpa_kv_dev(smc_ctx *ctx, const smc_kv *kv, const float *d_q, fl
  * Position p of sequence s is token p % page of page table[s * width + p / page].  `lengths` counts the tokens of a sequence, new ones included;
  * rows row_start[s] .. row_start[s + 1] - 1 of a call are its last ones (row_start null: one row each).  Rows from row_start[batch] on are
  * neither read nor written.  These arrays are on the device, so a captured CUDA graph serves what they hold when it is replayed.
+ * A sequence of length 0 is an empty slot, whatever rows it has (one, where row_start is null): the update writes nothing for them and passes their
+ * queries on as they are, the attention gives them zeros.
  * A page that a call writes belongs to one sequence; pages that are only read may be shared.  The calls queue on `stream` and keep nothing
- * in the context.  A page number outside of [0, pages), a length outside of the table or of the rotation's tables, or rows outside of the
- * call's raise smc_device_status (value 6): nothing is read or written outside of the arrays, the results of that sequence are not defined. */
+ * in the context.  A page number outside of [0, pages), a length outside of the table or of the rotation's tables, rows outside of the
+ * call's, or (the update) more rows than tokens where there are tokens raise smc_device_status (value 6): nothing is read or written outside of
+ * the arrays, the results of that sequence are not defined. */
 typedef struct smc_paged_kv {
     void *k, *v;   /* [pages, kv_heads, page, head_dim], [pages, kv_heads, head_dim, page], 16-byte aligned */
     float *scales; /* [pages, kv_heads, 2]: keys, values */

@@ -80,22 +80,23 @@ __global__ void __launch_bounds__(UPDATE_THREADS) paged_update_kernel(const Upda
         const int r = (int)(blockIdx.x - jobs), s = smc_paged_row_sequence(c, r);
         if (s < 0) return;
         const smc_paged_seq sq = smc_paged_sequence(c, s);
-        const int pos = sq.len - sq.n + r - sq.r0;
+        const bool empty = sq.len == 0 && !sq.bad;  // an empty slot's queries go through as they are
+        const int pos = empty ? 0 : sq.len - sq.n + r - sq.r0, rope_dim = empty ? 0 : u.rope_dim;
         if (pos < 0 || pos >= u.table_rows) {
             if (u.cosT && tid == 0) *u.status = SMC_STATUS_PAGED;
             return;
         }
-        const float *cs = u.cosT + (size_t)pos * (u.rope_dim >> 1), *sn = u.sinT + (size_t)pos * (u.rope_dim >> 1);
+        const float *cs = u.cosT + (size_t)pos * (rope_dim >> 1), *sn = u.sinT + (size_t)pos * (rope_dim >> 1);
         const T *src = static_cast<const T *>(u.q) + (long long)r * u.q_stride;
         T *dst = static_cast<T *>(u.q_out) + (long long)r * u.heads * HD;
 #pragma unroll 2
         for (int i = tid; i < u.heads * UNITS; i += UPDATE_THREADS) {  // (in place: a unit is read and written by one thread)
             const int h = i / UNITS;
             int first, second;
-            unit_place(i % UNITS, u.rope_dim, u.neox, first, second);
+            unit_place(i % UNITS, rope_dim, u.neox, first, second);
             float a[4], b[4];
             smc_paged_load4(src + h * HD + first, a), smc_paged_load4(src + h * HD + second, b);
-            unit_rotate(a, b, first, u.rope_dim, u.neox, cs, sn);
+            unit_rotate(a, b, first, rope_dim, u.neox, cs, sn);
             smc_paged_store4(dst + h * HD + first, a), smc_paged_store4(dst + h * HD + second, b);
         }
         return;
@@ -114,6 +115,7 @@ __global__ void __launch_bounds__(UPDATE_THREADS) paged_update_kernel(const Upda
     }
     const smc_paged_seq sq = smc_paged_sequence(c, s);
     const int p0 = sq.len - sq.n;
+    if (sq.len == 0 && !sq.bad) return;
     if (sq.bad || p0 < 0 || (u.cosT && sq.len > u.table_rows)) {
         if (tid == 0) *u.status = SMC_STATUS_PAGED;
         return;

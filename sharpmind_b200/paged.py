@@ -4,7 +4,8 @@ header).  The reference's caches are contiguous (SharpMind.Model/IKVCache.cs); t
 
 The memory is three tensors of the caller's (`PagedKVCache.create` makes them), and which page belongs to which
 sequence is the caller's too: every call takes the page table, the lengths (new tokens included) and, where sequences have
-other than one row each, the rows' starts, all int32 tensors on the device.  No call waits for the device, and a captured
+other than one row each, the rows' starts, all int32 tensors on the device.  A sequence of length 0 is an empty slot: `Update` writes
+nothing for its rows and passes their queries on as they are, `attention` gives them zeros.  No call waits for the device, and a captured
 CUDA graph serves whatever these tensors hold when it is replayed.
 """
 from __future__ import annotations
