@@ -24,7 +24,7 @@
 
 namespace {
 
-constexpr int RUNS_MOST = 1024, PART = 16, PARTS_MOST = 4, PART_TILES = 16;
+constexpr int RUNS_MOST = 1024, PART = 16, PARTS_MOST = 4, PART_TILES = 15;
 constexpr int WARPS = 4, THREADS = 32 * WARPS, UNIT = 64, SLOTS = 3, CHUNKS = 256;
 constexpr float W_SHIFT = 14.0f, W_UP = 64.0f, W_DOWN = 0x1p-64f, LOW = -60.0f;
 
@@ -521,9 +521,15 @@ int runs_for(const smc_ctx *ctx, int kvh, int batch, int parts, int max_len)
 
 }  // namespace
 
-// A part costs a pass over the keys, from L2 but for the first, where the tcgen05 form takes 256 pairs at once: up to four parts, and sixteen tiles of keys for each
-// (bf16, here / there: 20 pairs, 64 sequences of up to 8000 keys 259 / 555 us, of up to 2000 108 / 157, one of 500 19 / 16; 35 pairs, 64 of 2000 57 / 49, of 3000
-// 60 / 73; 64 pairs, 64 of 3000 258 / 224, of 4000 254 / 276, but in fp32 354 / 308, of 8000 336 / 524).  Up to 16 pairs: 16, one sequence of 500 12 / 16 us, 64 of 8000 151 / 523.
+// A part costs a pass over the keys, from L2 but for the first, where the tcgen05 form takes 256 pairs at once: up to four parts, and fifteen tiles of keys for each.
+// Here / there in us, 8 KV heads of 128, sequences of up to so many keys:
+//            one sequence         8                    24                   64
+//   20 pairs  2000: 14 / 19, 8000: 22 / 26    2000: 28 / 44, 8000: 47 / 106    2000: 58 / 85, 8000: 129 / 264    2000: 109 / 158, 8000: 266 / 555
+//   48        2000: 17 / 20, 8000: 27 / 27    2000: 34 / 44, 3000: 34 / 49     2000: 79 / 76, 3000:  87 / 123    2000: 161 / 165, 3000: 183 / 238
+//   64        4000: 25 / 24, 8000: 30 / 28    2000: 37 / 42, 4000: 39 / 65     3000: 103 / 118, 4000: 140 / 153  3000: 262 / 224, 4000: 261 / 277
+//   64 fp32   4000: 31 / 30, 8000: 37 / 34    2000: 45 / 45, 4000: 50 / 76     3000: 130 / 132, 4000: 178 / 170  3000: 333 / 251, 4000: 342 / 308, 6000: 377 / 429
+// So 64 pairs of one sequence lose 1 to 3 us by the rule, and 64 fp32 ones of 64 sequences of some 4000 lose 34; few sequences with 33 and more pairs would gain from half as many tiles.
+// Up to 16 pairs: 16, one sequence of 500 12 / 16 us, 64 of 8000 151 / 523.
 bool smc_paged_decode_takes(int group, int max_rows, int max_len)
 {
     const long long pairs = (long long)max_rows * group;

@@ -53,9 +53,9 @@ def put_codes(p, exponents, tag):
 
 
 def is_many(rows, group, length):
-    """The form that a call of one sequence takes: up to 16 pairs the one of a few rows, up to 64 where there are sixteen tiles of 64 keys for each 16 of them."""
+    """The form that a call of one sequence takes: up to 16 pairs the one of a few rows, up to 64 where there are fifteen tiles of 64 keys for each 16 of them."""
     pairs = rows * group
-    return not (pairs <= 16 or (pairs <= 64 and -(-length // 64) >= 16 * -(-pairs // 16)))
+    return not (pairs <= 16 or (pairs <= 64 and -(-length // 64) >= 15 * -(-pairs // 16)))
 
 
 ORDERS = {

@@ -11,6 +11,19 @@ pytestmark = pytest.mark.gpu
 F32, BF16 = torch.float32, torch.bfloat16
 
 
+def test_calls_of_some_pairs_take_the_form_that_was_measured_faster(cuda):
+    """The work space tells the forms apart: runs of sixteen pairs ask for less than pieces of 256.  3 x 16 pairs over 3000 keys and 4 x 16 over 4000 go by sixteens,
+    over 2000 and 3000 they do not."""
+    kv = paged._Kv(256, 256, 256, 1, 8, 64, 128)
+
+    def need(rows, length):
+        return cuda.lib.smc_paged_attention_work(cuda.h, C.byref(kv), 8, 8 * rows, 32, rows, length)
+
+    runs = need(16, 8000)
+    for rows, length, sixteens in [(12, 3000, True), (16, 4000, True), (5, 2000, True), (12, 2000, False), (16, 3000, False)]:
+        assert (need(rows, length) <= runs) == sixteens, (rows, length)
+
+
 # heads, rows of a sequence, sequences, tokens: runs with a join, segments of sixteen pairs, pieces of a prompt, and calls that need none
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("heads,each,batch,length,needs", [(8, 1, 2, 5000, True), (8, 2, 3, 3000, True), (8, 16, 2, 4500, True), (8, 40, 2, 2000, True), (8, 1, 2, 400, False),
