@@ -379,9 +379,9 @@ SMC_API int smc_sdpa_kv_dev(smc_ctx *ctx, const smc_kv *kv, const float *d_q, fl
  * A sequence of length 0 is an empty slot, whatever rows it has (one, where row_start is null): the update writes nothing for them and passes their
  * queries on as they are, the attention gives them zeros.
  * A page that a call writes belongs to one sequence; pages that are only read may be shared.  The calls queue on `stream` and keep nothing
- * in the context.  A page number outside of [0, pages), a length outside of the table or of the rotation's tables, rows outside of the
- * call's, or (the update) more rows than tokens where there are tokens raise smc_device_status (value 6): nothing is read or written outside of
- * the arrays, the results of that sequence are not defined. */
+ * in the context.  A page number outside of [0, pages), a length outside of the table or of the rotation's tables or above 2^31 - 256, rows
+ * outside of the call's, or (the update) more rows than tokens where there are tokens raise smc_device_status (value 6): nothing is read or
+ * written outside of the arrays, the results of that sequence are not defined. */
 typedef struct smc_paged_kv {
     void *k, *v;   /* [pages, kv_heads, page, head_dim], [pages, kv_heads, head_dim, page], 16-byte aligned */
     float *scales; /* [pages, kv_heads, 2]: keys, values */

@@ -30,7 +30,7 @@ __device__ __forceinline__ smc_paged_seq smc_paged_sequence(const smc_paged_view
     q.r0 = min(max(a, 0), c.rows);
     q.n = min(max(b, q.r0), c.rows) - q.r0;
     const int len = c.lengths[s];
-    const long long most = (long long)c.width << c.shift;
+    const long long most = min((long long)c.width << c.shift, 0x7FFFFF00LL);  // (a few tiles of keys behind a length are still an int)
     q.len = (int)min((long long)max(len, 0), most);
     q.bad = a < 0 || b < a || b > c.rows || len < 0 || len > most;
     return q;

@@ -5,9 +5,9 @@ import math
 import pytest
 import torch
 
-from sharpmind_b200 import paged  # noqa: F401
+from sharpmind_b200 import ops
 from tests import paged_util
-from tests.test_gpu_paged import Pair, gen, ints, randn, starts
+from tests.test_gpu_paged import Pair, gen, ints, near, randn, starts
 
 pytestmark = pytest.mark.gpu
 F32, BF16 = torch.float32, torch.bfloat16
@@ -139,3 +139,54 @@ def test_all_the_weight_on_a_key_of_a_small_block(cuda, dtype, rows, length):
     big = want.abs() > 2.0 ** -20
     assert float(big.double().mean()) > 0.9 and bool((bound[big] < 0.1 * want[big].abs()).all()), "the bound is to see a result that vanishes"
     assert bool(((got - want).abs() <= bound).all()), float(((got - want).abs() / bound).max())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,length", [(1, 450), (4, 6000), (16, 4500), (200, 450), (70, 3000)])
+@pytest.mark.parametrize("size", [1e4, 1e6, 1e7])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_of_large_magnitude(cuda, dtype, rows, length, size, sign):
+    """Scores up to `size`, all of one sign, the nearest ones apart by more than fp32 rounds: the values of the largest, or the mean of those that share it.
+
+    Queries and keys have one dimension other than 0, so scores are exact but for the roundings that equal ones share; the value scales are equal.  What is left of the
+    bound: the sums and the exponential, and the roundings to 11 bits and of the result."""
+    dim, heads = 64, 4
+    p = Pair(cuda, [length], page=16, dim=dim, tag="large")
+    p.plain.k[:] = 0
+    p.plain.k[..., 7] = torch.randint(0x70, 0x7F, p.plain.k.shape[:3], dtype=torch.uint8, generator=gen("large", length))  # 128 .. 448, steps of an eighth or less
+    p.plain.v[:] = torch.randint(0, 112, p.plain.v.shape, dtype=torch.uint8, generator=gen("large v", length))
+    p.plain.scales[..., 0], p.plain.scales[..., 1] = 64.0, 0.5
+    p.upload()
+    q = torch.zeros((rows, heads, dim))
+    q[:, :, 7] = sign * size / (448 * 64 * 0.125)
+    q = q.to(dtype)
+    got = p.cache.attention(q.cuda(), p.dtable, ints([length]), 0.125, row_start=starts([rows]), max_rows=rows, max_len=length).cpu().double()
+    k, v = p.plain.tokens(p.table[0], length)
+    for r in range(rows):
+        seen = length - rows + r + 1
+        for h in range(heads):
+            x = k[:seen, h // 2, 7] * float(q[r, h, 7])
+            top = x == x.max()
+            want, spread = v[:seen, h // 2][top].mean(0), v[:seen, h // 2][top].abs().mean(0)
+            bound = (length * 2.0 ** -23 + 2.0 ** -19) * spread + (2.0 ** -11 * spread + 2.0 ** -8 * want.abs() if dtype == BF16 else 0.0)
+            assert bool(((got[r, h] - want).abs() <= bound).all()), (r, h)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 150])
+def test_lengths_near_two_to_the_31(cuda, rows):
+    """The last tokens of a sequence of 2^31 - 256, seen through a window, are those of a short one; a longer one raises the status."""
+    page, dim, window, tail = 64, 64, 400, 12
+    p = Pair(cuda, [tail * page], page=page, dim=dim)
+    p.fill([tail * page])
+    length = 2 ** 31 - 256
+    table = torch.zeros((1, 2 ** 31 // page), dtype=torch.int32, device="cuda")
+    table[0, length // page - tail:length // page] = p.dtable[0, :tail]
+    q = randn((rows, 4, dim), "end", rows)
+    args = dict(row_start=starts([rows]), max_rows=rows, window=window)
+    for most in (length, 1000):
+        got = p.cache.attention(q.cuda(), table, ints([length]), 0.125, max_len=most, **args)
+        near(got, q, p, [tail * page], [rows], 0.125, window)
+    assert cuda.device_status() == 0
+    p.cache.attention(q.cuda(), table, ints([2 ** 31 - 1]), 0.125, max_len=1000, **args)
+    with pytest.raises(ops.SharpMindCudaError, match="status 6"):
+        cuda.device_status()
