@@ -406,7 +406,10 @@ SMC_API int smc_paged_read_dev(smc_ctx *ctx, const smc_paged_kv *kv, const int *
  * [rows, heads, head_dim] with a row stride in elements, d_out contiguous, both of `dtype`.  window > 0: position i sees
  * i - window + 1 .. i.  A row that sees no key gets zeros.  max_rows bounds the rows of a sequence (one with more raises status 6) and max_len says how
  * long the sequences may be; both are known to the host and choose and size the launch.  d_work: smc_paged_attention_work bytes (-1 for
- * bad arguments), 16-byte aligned, used by this call alone until it has completed. */
+ * bad arguments), 16-byte aligned, used by this call alone until it has completed.
+ * Scores may be up to 1e7 in magnitude (beyond, a row may come out undefined).  Weights are fp32 in the softmax's sum.  In the product with the
+ * values they are fp16 (fp32 rows: two parts): off by 2^-11 (2^-22) of themselves, or where that is more by 2^-31 of the row's largest weight times value
+ * scale, 2^-39 in the form for up to 16 pairs of a row and a query head of one KV head (up to 64 over long caches). */
 SMC_API int64_t smc_paged_attention_work(smc_ctx *ctx, const smc_paged_kv *kv, int batch, int rows, int heads, int max_rows, int max_len);
 SMC_API int smc_paged_attention_dev(smc_ctx *ctx, const smc_paged_kv *kv, const smc_paged_seqs *seqs, int dtype, const void *d_q, long long q_stride, void *d_out,
                                     int heads, float scale, int window, int max_rows, int max_len, void *d_work, long long work_bytes, void *stream);

@@ -11,7 +11,7 @@
 // A warp's unit: keys and values arrive by bulk copies in a ring of its own, K or V of 64 tokens a slot, two slots ahead.  Scores and outputs
 // are mma.sync m16n8k16 in fp16 with fp32 sums, transposed: S^T = K Q^T and O^T = V^T P^T, so that the eight columns are the (row, query head) pairs, of which
 // there are few, and no tile is half empty.  An e4m3 code is exact in fp16; the queries are scaled by a power of two per row to 2^15 at most, which bfloat16
-// ones take exactly; fp32 queries and weights go in as hi + lo, 22 bits, into the same sums.
+// ones take exactly; fp32 queries and weights go in as hi + lo, 22 bits (weights as long as they are 2^-3 or more, 2^-17 of the largest), into the same sums.
 // Both products' contraction indices are permuted so that a thread reads 16 contiguous codes: thread t of a quad takes dims [16 t, 16 t + 16) (and + 64) of
 // the keys, tokens [16 t, 16 t + 16) of the values.  The scores' row i of tile pair M is token 16 (i / 2) + 2 M + i % 2: a transposed eight by eight
 // block of weights (movmatrix) then is the second product's operand, and all tokens of a thread's scores lie in one page, so a unit's scales are two numbers.

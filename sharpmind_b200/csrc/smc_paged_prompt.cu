@@ -4,10 +4,11 @@
 // they lie in their pages, turned to fp16 (exact) by four warps and stored as 128-byte-swizzled K-major tiles, once for all heads of a group and both
 // tiles.  Scores S = Q K^T and outputs O += P V are tcgen05.mma, fp16 with fp32 sums in tensor memory, P in the columns that S leaves:
 //   bfloat16  queries exact in fp16 after a power of two per row, weights rounded to 11 bits
-//   fp32      queries and weights as hi + lo, 22 bits, two products each
+//   fp32      queries and weights as hi + lo, two products each: 22 bits, of weights as long as they are 2^-3 or more (lo, too, goes in steps of 2^-24)
 // With the pages' scales, constant over 16 keys:  y = S f + b, f = s_k * row factor, b = log2(s_v);  w = 2^(y - R);  l = sum w / s_v;  out = O / l.
 // R is 6 below the maximum of y of a row's first step and goes up (to 6 below the maximum) only where a step's weights sum up to more than fp16 holds: a step takes
-// no maximum, and O, in tensor memory, is rarely multiplied again.  A weight counts down to 2^-24, 2^-30 of the largest of the first step.
+// no maximum, and O, in tensor memory, is rarely multiplied again.  What is left below a weight's last step, 2^-25 at most, is lost to O: 2^-31 of the largest of the first step, in
+// both types (a first key that takes all but 2^-20 of the weight and has no value leaves the others 11 bits each).  The sum l loses nothing: its weights are fp32.
 // Warp roles:  0 .. 3, 4 .. 7  softmax of tile 0, 1      8 .. 11  codes to fp16      12, 13  MMA issue of tile 0, 1
 // Scores have two buffers a tile, so a softmax finds its next ones there.
 // Few pairs: the steps are split over CTAs, whose partial results a second kernel joins.
