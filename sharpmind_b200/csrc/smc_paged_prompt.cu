@@ -12,8 +12,8 @@
 // Warp roles:  0 .. 3, 4 .. 7  softmax of tile 0, 1      8 .. 11  codes to fp16      12, 13  MMA issue of tile 0, 1
 // Scores have two buffers a tile, so a softmax finds its next ones there.
 // Few pairs: the steps are split over CTAs, whose partial results a second kernel joins.
-// Measured (6000 bf16 rows, 32 query heads, 8 of keys, of 128): 391 us, 754 TFLOP/s, 45 % of a bf16 matmul's rate; 1.46 us a step.  Tensor pipe 30 % active, issue slots 42 %: the chain from scores to weights
-// bounds it, no unit.  Leaving out the exponentials gained 1 %, all MMAs 7 %, the stores of the converted tiles 11 %.
+// Measured (6000 bf16 rows, 32 query heads, 8 of keys, of 128): 394 us, 748 TFLOP/s, 44 % of a bf16 matmul's rate; 1.46 us a step.  With 3000 rows the tensor pipe is active 30 % of the time and issue
+// slots 41 %: the chain from scores to weights bounds it, no unit.  Leaving out the exponentials gained 1 %, all MMAs 7 %, the stores of the converted tiles 11 %.
 #include "smc_paged.cuh"
 #include "smc_tc.cuh"
 
